@@ -14,6 +14,8 @@ from . import build as _build
 OK = 0
 ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE, ERR_NOMEM = -1, -2, -3, -4, -5
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+
 _i32p = C.POINTER(C.c_int32)
 _vp = C.c_void_p
 
@@ -36,6 +38,14 @@ SIGNATURES = {
     "aiehlc_srs_i32_i8_dev": (C.c_int, [_vp, _vp, _vp, C.c_longlong, C.c_longlong, C.c_int, _vp, _vp]),
     "aiehlc_gemm_bf16_dev": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp]),
     "aiehlc_gemm_bf16_host": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int]),
+    "aiehlc_mxfp4_pitch": (C.c_longlong, [C.c_longlong]),
+    "aiehlc_mxfp4_scale_bytes": (C.c_longlong, [C.c_longlong, C.c_longlong]),
+    "aiehlc_quantize_mxfp4_dev": (C.c_int, [_vp, _vp, C.c_int, C.c_longlong, C.c_longlong, C.c_longlong, _vp, _vp, _vp,
+                                            _vp, _vp]),
+    "aiehlc_dequantize_mxfp4_dev": (C.c_int, [_vp, _vp, _vp, C.c_longlong, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp]),
+    "aiehlc_gemm_mxfp4_dev": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_longlong,
+                                        C.c_int, _vp]),
+    "aiehlc_gemm_mxfp4_mxfp4_dev": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp]),
     "aiehlc_conv2d_i8_srs_dev": (C.c_int, [_vp, _vp, _vp, _vp] + [C.c_int] * 8 + [_vp, _vp]),
     "aiehlc_conv2d_i8_srs_host": (C.c_int, [_vp, _vp, _vp, _vp] + [C.c_int] * 8 + [_vp]),
     "aiehlc_conv2d_pack_weights_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),

@@ -24,7 +24,7 @@ OBJ_DIR = PKG / ("_obj_measure" if MEASURE else "_obj")
 LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / ("libaiehlc_b200_measure.so" if MEASURE else "libaiehlc_b200.so")
 
-CUDA_SOURCES = ["capi.cu", "gemm_launch.cu", "simt_kernels.cu", "conv_tcgen05.cu"]
+CUDA_SOURCES = ["capi.cu", "gemm_launch.cu", "simt_kernels.cu", "conv_tcgen05.cu", "mxfp4_quant.cu", "mxfp4_gemm.cu"]
 CXX_SOURCES = ["xaie_runtime.cpp"]
 
 NVCC_FLAGS = [

@@ -9,6 +9,7 @@
 #include "../../include/aiehlc_b200_tuning.h"
 #include "context.h"
 #include "gemm_tcgen05.cuh"
+#include "mxfp4.cuh"
 
 namespace aiehlc {
 
@@ -498,6 +499,107 @@ int aiehlc_gemm_bf16_dev(aiehlc_ctx* ctx, const uint16_t* A, const uint16_t* B, 
   c.kind = KIND_BF16; c.epi = EPI_BF16;
   c.A = A; c.B = B; c.C = C; c.M = M; c.N = N; c.K = K; c.lda = K; c.ldb = K; c.ldc = N;
   return launch_gemm(ctx, c, st);
+}
+
+// ------------------------------------------------------------------ microscaled 4-bit matrices
+long long aiehlc_mxfp4_pitch(long long cols) { return cols > 0 ? mx_pitch(cols) : 0; }
+long long aiehlc_mxfp4_scale_bytes(long long rows, long long cols) {
+  return rows > 0 && cols > 0 ? mx_scale_bytes(rows, cols) : 0;
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+static int type_bytes(int type) { return type == AIEHLC_TYPE_F32 ? 4 : 2; }
+static int check_mx_matrix(const void* x, int type, long long rows, long long cols, long long ld, const char* what) {
+  const std::string op(what);
+  if (type < AIEHLC_TYPE_F32 || type > AIEHLC_TYPE_F16) return fail(AIEHLC_ERR_INVALID, op + ": unknown type");
+  if (rows < 0 || cols < 0) return fail(AIEHLC_ERR_INVALID, op + ": negative size");
+  if (ld < cols) return fail(AIEHLC_ERR_INVALID, op + ": the row pitch is shorter than a row");
+  if (rows == 0 || cols == 0) return AIEHLC_OK;
+  if (!x) return fail(AIEHLC_ERR_INVALID, op + ": null matrix");
+  if (reinterpret_cast<uintptr_t>(x) % type_bytes(type) != 0) return fail(AIEHLC_ERR_INVALID, op + ": misaligned matrix");
+  // one CTA per 128 x 128 tile
+  const long long high = (rows - 1) / 128 + 1, wide = (cols - 1) / 128 + 1;
+  if (high > 0x7FFFFFFFLL || wide > 0x7FFFFFFFLL / high) return fail(AIEHLC_ERR_UNSUPPORTED, op + ": more than 2^31 tiles of 128 x 128");
+  return AIEHLC_OK;
+}
+static int check_mx_codes(const void* codes, const void* scales, const char* what) {
+  if (!codes || !scales) return fail(AIEHLC_ERR_INVALID, std::string(what) + ": null codes or scales");
+  if (!aligned16(codes) || !aligned16(scales))
+    return fail(AIEHLC_ERR_INVALID, std::string(what) + ": codes and scales must be 16-byte aligned");
+  return AIEHLC_OK;
+}
+
+int aiehlc_quantize_mxfp4_dev(aiehlc_ctx* ctx, const void* x, int type, long long rows, long long cols, long long ld,
+                              uint8_t* q, uint8_t* q_scales, uint8_t* t, uint8_t* t_scales, void* stream) {
+  int rc = check_mx_matrix(x, type, rows, cols, ld, "quantize_mxfp4");
+  if (rc) return rc;
+  const bool empty = rows == 0 || cols == 0;
+  if (!empty && !q && !q_scales && !t && !t_scales) return fail(AIEHLC_ERR_INVALID, "quantize_mxfp4: no output");
+  if (!empty && (q || q_scales) && (rc = check_mx_codes(q, q_scales, "quantize_mxfp4 (rows)"))) return rc;
+  if (!empty && (t || t_scales) && (rc = check_mx_codes(t, t_scales, "quantize_mxfp4 (columns)"))) return rc;
+  if ((rc = check_ctx(ctx)) || empty) return rc;
+  return launch_mx_quantize(ctx, MxQuantizeCall{x, type, rows, cols, ld, q, q_scales, t, t_scales}, pick_stream(ctx, stream));
+}
+
+int aiehlc_dequantize_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* q, const uint8_t* q_scales, long long rows, long long cols,
+                                void* y, int type, long long ld, void* stream) {
+  int rc = check_mx_matrix(y, type, rows, cols, ld, "dequantize_mxfp4");
+  if (rc) return rc;
+  const bool empty = rows == 0 || cols == 0;
+  if (!empty && (rc = check_mx_codes(q, q_scales, "dequantize_mxfp4"))) return rc;
+  if ((rc = check_ctx(ctx)) || empty) return rc;
+  return launch_mx_dequantize(ctx, q, q_scales, rows, cols, y, type, ld, pick_stream(ctx, stream));
+}
+
+static int check_mx_product(const void* A, const void* As, const void* B, const void* Bs, int K, const char* what) {
+  if (K == 0) return AIEHLC_OK;
+  if (int rc = check_mx_codes(A, As, what)) return rc;
+  return check_mx_codes(B, Bs, what);
+}
+static int check_mx_sizes(int M, int N, int K, const char* what) {
+  if (M < 0 || N < 0 || K < 0) return fail(AIEHLC_ERR_INVALID, std::string(what) + ": negative size");
+  if (M > 1 << 30 || N > 1 << 30 || K > 1 << 30) return fail(AIEHLC_ERR_UNSUPPORTED, std::string(what) + ": M, N, K up to 2^30");
+  // one CTA (or pair) per output tile, at most eight times as many with K split
+  if ((M / 128 + 1LL) * (N / 128 + 1LL) > 1LL << 28) return fail(AIEHLC_ERR_UNSUPPORTED, std::string(what) + ": too many output tiles");
+  return AIEHLC_OK;
+}
+
+int aiehlc_gemm_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* A, const uint8_t* A_scales, const uint8_t* B,
+                          const uint8_t* B_scales, void* C, int type, int M, int N, int K, long long ldc, int accumulate,
+                          void* stream) {
+  if (type < AIEHLC_TYPE_F32 || type > AIEHLC_TYPE_F16) return fail(AIEHLC_ERR_INVALID, "gemm_mxfp4: unknown type");
+  int rc = check_mx_sizes(M, N, K, "gemm_mxfp4");
+  if (rc) return rc;
+  if (accumulate && type != AIEHLC_TYPE_F32) return fail(AIEHLC_ERR_UNSUPPORTED, "gemm_mxfp4: only f32 results can be added to C");
+  if (ldc < N) return fail(AIEHLC_ERR_INVALID, "gemm_mxfp4: the row pitch of C is shorter than a row");
+  const bool empty = M == 0 || N == 0;
+  if (!empty && (!C || reinterpret_cast<uintptr_t>(C) % type_bytes(type) != 0))
+    return fail(AIEHLC_ERR_INVALID, "gemm_mxfp4: null or misaligned C");
+  if (!empty && (rc = check_mx_product(A, A_scales, B, B_scales, K, "gemm_mxfp4"))) return rc;
+  if ((rc = check_ctx(ctx)) || empty) return rc;
+  cudaStream_t st = pick_stream(ctx, stream);
+  if (K == 0) {
+    if (!accumulate) AIEHLC_CUDA(cudaMemset2DAsync(C, static_cast<size_t>(ldc) * type_bytes(type), 0, static_cast<size_t>(N) * type_bytes(type), M, st));
+    return AIEHLC_OK;
+  }
+  return launch_mx_gemm(ctx, MxGemmCall{A, A_scales, B, B_scales, C, nullptr, type, accumulate ? 1 : 0, M, N, K, ldc}, st);
+}
+
+int aiehlc_gemm_mxfp4_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* A, const uint8_t* A_scales, const uint8_t* B,
+                                const uint8_t* B_scales, uint8_t* C, uint8_t* C_scales, int M, int N, int K, void* stream) {
+  int rc = check_mx_sizes(M, N, K, "gemm_mxfp4_mxfp4");
+  if (rc) return rc;
+  const bool empty = M == 0 || N == 0;
+  if (!empty && (rc = check_mx_codes(C, C_scales, "gemm_mxfp4_mxfp4 (C)"))) return rc;
+  if (!empty && (rc = check_mx_product(A, A_scales, B, B_scales, K, "gemm_mxfp4_mxfp4"))) return rc;
+  if ((rc = check_ctx(ctx)) || empty) return rc;
+  cudaStream_t st = pick_stream(ctx, stream);
+  if (K == 0) {
+    AIEHLC_CUDA(cudaMemsetAsync(C, 0, static_cast<size_t>(M) * mx_pitch(N), st));
+    AIEHLC_CUDA(cudaMemsetAsync(C_scales, 0, static_cast<size_t>(mx_scale_bytes(M, N)), st));
+    return AIEHLC_OK;
+  }
+  return launch_mx_gemm(ctx, MxGemmCall{A, A_scales, B, B_scales, C, C_scales, AIEHLC_TYPE_F32, 0, M, N, K, N}, st);
 }
 
 int aiehlc_conv2d_i8_srs_dev(aiehlc_ctx* ctx, const int8_t* x, const int8_t* w, int8_t* y, int n, int h, int wd,

@@ -155,6 +155,27 @@ int launch_fill_i32(aiehlc_ctx* ctx, int32_t* out, long long n, int value, cudaS
 int launch_repack(aiehlc_ctx* ctx, const void* src, void* dst, long long rows, long long cols,
                   long long ld_src, long long ld_dst, int esize, cudaStream_t st);
 
+// microscaled 4-bit matrices (mxfp4_quant.cu, mxfp4_gemm.cu; format: mxfp4.cuh).  Arguments have been checked.
+struct MxQuantizeCall {
+  const void* x;
+  int type;
+  long long rows, cols, ld;
+  uint8_t* q; uint8_t* qs;      // blocks along the rows, or null
+  uint8_t* t; uint8_t* ts;      // blocks along the columns (of the transposed matrix), or null
+};
+int launch_mx_quantize(aiehlc_ctx* ctx, const MxQuantizeCall& c, cudaStream_t st);
+int launch_mx_dequantize(aiehlc_ctx* ctx, const uint8_t* q, const uint8_t* qs, long long rows, long long cols, void* y,
+                         int type, long long ld, cudaStream_t st);
+struct MxGemmCall {
+  const uint8_t* A; const uint8_t* As;
+  const uint8_t* B; const uint8_t* Bs;
+  void* C; uint8_t* Cs;         // Cs: C is quantised too (codes in C), else null
+  int type, accumulate;
+  int M, N, K;
+  long long ldc;
+};
+int launch_mx_gemm(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st);
+
 // implicit-GEMM conv (conv_tcgen05.cu)
 // `weight_scratch`: where re-laid weights ([tap][cout][cin], kh*kw*cin*cout bytes) are kept when the
 // shape needs them; null = the context's growing workspace.

@@ -1,0 +1,340 @@
+// Products of microscaled 4-bit matrices (format: mxfp4.cuh) on the tcgen05 tensor cores, kind::mxf4:
+//     C[m][n] = sum_k A[m][k] * B[n][k],  each factor an e2m1 number times its block's power of two.
+// The products are exact, the sums are held in 32 bits (TMEM).  C leaves as f32 (optionally added to what is there),
+// bf16, f16, or quantised again along its rows.
+#include "context.h"
+#include "mxfp4.cuh"
+#include "sm100_ptx.cuh"
+
+namespace aiehlc {
+
+namespace {
+
+enum : int { MX_F32 = 0, MX_F32_ADD = 1, MX_BF16 = 2, MX_F16 = 3, MX_MX = 4 };
+
+constexpr int kStepK = 256;                    // elements of K per stage: one 128-byte swizzle span of codes
+constexpr int kStepScales = 2 * kMxScaleTile;  // two scale tiles of 4 blocks each
+constexpr int kMmaK = 64;                      // elements of K per tcgen05.mma
+
+struct MxGemmParams {
+  int M, N, K;
+  int k_steps;              // steps of 256 elements
+  int words;                // scale tiles along K (of 128 elements)
+  const uint8_t* a_scales;
+  const uint8_t* b_scales;
+  void* C;                  // f32 / bf16 / f16, leading dimension ldc; MX_MX: codes
+  uint8_t* c_scales;        // MX_MX
+  long long ldc;
+  int vec_ok;               // four results at a time may be stored as a vector
+  int m_tiles, n_tiles;
+  int* status;
+  int debug;                // 3: the producer withholds its loads, so every wait runs out
+};
+
+// ---------------------------------------------------------------------------------------- few rows of A
+// The rows of B are the 128 rows of the MMA and the rows of A its kTN columns, so that a product with few rows of A
+// streams B through as many SMs as there are: each output tile (128 columns of C x kTN rows) is one cluster of
+// `split` CTAs, each of which takes an equal range of K.  The partial sums meet in distributed shared memory, added in the order
+// of the CTAs' ranks (the result does not depend on timing), and every CTA writes its share of the tile's rows.
+template <int kTN>
+struct NarrowShape {
+  static constexpr int kStages = 4;
+  static constexpr int kBBytes = 128 * 128;
+  static constexpr int kABytes = kTN * 128;
+  static constexpr int kStageBytes = kBBytes + kABytes + 2 * kStepScales;
+  static constexpr int kPartialBytes = kTN * 128 * 4;         // over the stages, once they are done
+  static constexpr int kPool = kStages * kStageBytes > kPartialBytes ? kStages * kStageBytes : kPartialBytes;
+  static constexpr int kTotal = 1024 + kPool + 256;
+  static constexpr int kScaleCols = 32;                       // two sets of 8 columns for each operand
+  static constexpr int kTmemCols = kTN <= 32 ? 64 : kTN == 64 ? 128 : 256;
+  static_assert(kTN + kScaleCols <= kTmemCols, "TMEM");
+};
+
+// Stores four consecutive results of a row; `n` is the first one's column.
+template <int kOut>
+__device__ __forceinline__ void store4(const MxGemmParams& p, int m, int n, const float4& v) {
+  const long long at = static_cast<long long>(m) * p.ldc + n;
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (kOut == MX_F32 || kOut == MX_F32_ADD) {
+    float* c = static_cast<float*>(p.C) + at;
+    if (p.vec_ok && n + 4 <= p.N) {
+      float4 o = v;
+      if constexpr (kOut == MX_F32_ADD) {
+        const float4 was = *reinterpret_cast<const float4*>(c);
+        o.x += was.x; o.y += was.y; o.z += was.z; o.w += was.w;
+      }
+      *reinterpret_cast<float4*>(c) = o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.N) c[i] = kOut == MX_F32_ADD ? c[i] + f[i] : f[i];
+    }
+  } else {
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kOut == MX_BF16) h[i] = __bfloat16_as_ushort(__float2bfloat16_rn(f[i]));
+      else h[i] = __half_as_ushort(__float2half_rn(f[i]));
+    }
+    uint16_t* c = static_cast<uint16_t*>(p.C) + at;
+    if (p.vec_ok && n + 4 <= p.N) {
+      *reinterpret_cast<uint2*>(c) = make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.N) c[i] = h[i];
+    }
+  }
+}
+
+// The whole warp holds 128 consecutive results of row m, four per lane, first column n0 (a multiple of 128): four blocks
+// of eight lanes.  Writes their codes and the row's scale word.
+__device__ __forceinline__ void store_blocks(const MxGemmParams& p, int m, int n0, int lane, float4 v) {
+  const int n = n0 + 4 * lane;
+  float f[8] = {v.x, v.y, v.z, v.w, 0.0f, 0.0f, 0.0f, 0.0f};
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n + i >= p.N) f[i] = 0.0f;
+    most = max(most, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+  const int s = mx_scale_of(most);
+  const float inv = mx_inverse(s);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = mx_scaled(f[i], inv);
+  const uint16_t codes = static_cast<uint16_t>(mx_codes8(f));
+  const int blocks = static_cast<int>(mx_blocks(p.N));
+  const bool there = n / kMxBlock < blocks;
+  if (there) *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.C) + static_cast<long long>(m) * blocks * 16 + n / 2) = codes;
+  uint32_t word = static_cast<uint32_t>(there ? s : 0) << (8 * (lane >> 3));
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 16);
+  if (lane == 0)
+    *reinterpret_cast<uint32_t*>(p.c_scales + (static_cast<long long>(m / 128) * mx_words(p.N) + n0 / 128) * kMxScaleTile +
+                                 mx_scale_word(m & 127)) = word;
+}
+
+template <int kTN, int kOut>
+__global__ void __launch_bounds__(128)
+mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const MxGemmParams p) {
+  using S = NarrowShape<kTN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kPool);
+  uint64_t* empty_bar = full_bar + S::kStages;
+  uint64_t* done_bar = empty_bar + S::kStages;
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int split = gridDim.x / (p.m_tiles * p.n_tiles);
+  const int tile = blockIdx.x / split;
+  const int m0 = tile % p.m_tiles * kTN;
+  const int n0 = tile / p.m_tiles * 128;
+  const int k_first = static_cast<int>(static_cast<long long>(p.k_steps) * rank / split);
+  const int k_last = static_cast<int>(static_cast<long long>(p.k_steps) * (rank + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    mbar_init(smem_u32(done_bar), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(tmem_base_slot), S::kTmemCols);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (warp == 0 && lane == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint8_t* sa = p.a_scales + static_cast<long long>(m0 / 128) * p.words * kMxScaleTile;
+    const uint8_t* sb = p.b_scales + static_cast<long long>(n0 / 128) * p.words * kMxScaleTile;
+    for (int k = k_first; k < k_last; ++k) {
+      ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status, ST_TIMEOUT_EMPTY);
+      if (!ok) break;
+      if (p.debug != 3) {
+        const uint32_t bar = smem_u32(&full_bar[stage]);
+        const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
+        const uint32_t scale_bytes = (p.words - 2 * k < 2 ? 1 : 2) * kMxScaleTile;  // K may end inside the step
+        mbar_expect_tx(bar, S::kBBytes + S::kABytes + 2 * scale_bytes);
+        tma_load_2d(at, &tmap_b, bar, k * 128, n0);
+        tma_load_2d(at + S::kBBytes, &tmap_a, bar, k * 128, m0);
+        bulk_load_g2s(at + S::kBBytes + S::kABytes, sb + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
+        bulk_load_g2s(at + S::kBBytes + S::kABytes + kStepScales, sa + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
+      }
+      if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+    }
+    if (!ok)
+      for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land before the CTA retires
+  } else if (warp == 1 && lane == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int k = k_first; k < k_last; ++k) {
+      ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
+      const uint32_t scales = at + S::kBBytes + S::kABytes;
+      const uint32_t t_scales = tmem_base + kTN + (k & 1) * 16;  // 8 columns of B's scales, 8 of A's
+      const int mmas = min(kStepK, p.K - k * kStepK + kMmaK - 1) / kMmaK;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (2 * w < mmas) {
+          tmem_copy_scales<1>(t_scales + 4 * w, make_scale_desc(scales + w * kMxScaleTile));
+          tmem_copy_scales<1>(t_scales + 8 + 4 * w, make_scale_desc(scales + kStepScales + w * kMxScaleTile));
+        }
+      const uint64_t bdesc = make_kmajor_desc(at, 1024, 2);
+      const uint64_t adesc = make_kmajor_desc(at + S::kBBytes, 1024, 2);
+#pragma unroll
+      for (int i = 0; i < kStepK / kMmaK; ++i)
+        if (i < mmas)
+          umma_mxf4<1>(tmem_base, bdesc + 2 * i, adesc + 2 * i, make_idesc_mxf4(128, kTN, 2 * (i & 1)),
+                       t_scales + 4 * (i >> 1), t_scales + 8 + 4 * (i >> 1), (k > k_first || i > 0) ? 1u : 0u);
+      umma_commit(smem_u32(&empty_bar[stage]));
+      if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+    }
+    if (ok) umma_commit(smem_u32(done_bar));
+  }
+  __syncwarp();
+
+  // Every warp turns its 32 rows of the accumulator (columns of C) into rows of 128 floats [row of C][column of C].
+  bool ok = mbar_wait(smem_u32(done_bar), 0, abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
+  ok = __all_sync(0xFFFFFFFFu, ok);
+  const int valid = min(kTN, p.M - m0);
+  float* partial = reinterpret_cast<float*>(smem);
+  if (ok) {
+    tc_fence_after();
+#pragma unroll
+    for (int c = 0; c < kTN; c += 16) {
+      if (c < valid) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) partial[(c + j) * 128 + warp * 32 + lane] = __uint_as_float(r[j]);
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // every CTA's partial sums are in place (one CTA: a barrier over its warps)
+
+  if (ok) {
+    const int first = valid * rank / split, last = valid * (rank + 1) / split;
+    const uint32_t mine = smem_u32(partial) + lane * 16;
+    for (int j = first + warp; j < last; j += 4) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int c = 0; c < split; ++c) {
+        const float4 o = ld_cluster_f4(mapa_u32(mine + j * 512, c));
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      }
+      if constexpr (kOut == MX_MX) store_blocks(p, m0 + j, n0, lane, v);
+      else if (n0 + 4 * lane < p.N) store4<kOut>(p, m0 + j, n0 + 4 * lane, v);
+    }
+    if constexpr (kOut == MX_MX) {
+      // rows of the last scale tile that do not exist
+      if (rank == 0 && m0 + kTN >= p.M)
+        for (int m = p.M + threadIdx.x; m < (p.M + 127) / 128 * 128; m += 128)
+          *reinterpret_cast<uint32_t*>(p.c_scales + (static_cast<long long>(m / 128) * mx_words(p.N) + n0 / 128) * kMxScaleTile +
+                                       mx_scale_word(m & 127)) = 0;
+    }
+  }
+  cluster_sync_all();  // the others may still read this CTA's partial sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, S::kTmemCols);
+  }
+}
+
+int encode_codes_map(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* codes, long long rows, long long cols, int box_rows) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(mx_pitch(cols)), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(mx_pitch(cols))};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AIEHLC_ERR_CUDA, "cuTensorMapEncodeTiled failed for the codes of a 4-bit operand");
+  return AIEHLC_OK;
+}
+
+template <int kTN, int kOut>
+int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStream_t st) {
+  using S = NarrowShape<kTN>;
+  CUtensorMap ma, mb;
+  if (int rc = encode_codes_map(ctx, &ma, c.A, c.M, c.K, kTN)) return rc;
+  if (int rc = encode_codes_map(ctx, &mb, c.B, c.N, c.K, 128)) return rc;
+  p.m_tiles = (c.M + kTN - 1) / kTN;
+  p.n_tiles = (c.N + 127) / 128;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  auto kern = mx_gemm_narrow_kernel<kTN, kOut>;
+  KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
+  if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::kTotal, &ks.smem_attr)) return rc;
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 2 * ctx->usable_sms() && split * 4 <= p.k_steps) split *= 2;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = S::kTotal;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctx->pdl ? 2 : 1;
+  AIEHLC_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, p));
+  ctx->launches++;
+  return AIEHLC_OK;
+}
+
+template <int kOut>
+int launch_out(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
+  MxGemmParams p{};
+  p.M = c.M; p.N = c.N; p.K = c.K;
+  p.k_steps = (c.K + kStepK - 1) / kStepK;
+  p.words = static_cast<int>(mx_words(c.K));
+  p.a_scales = c.As; p.b_scales = c.Bs;
+  p.C = c.C; p.c_scales = c.Cs; p.ldc = c.ldc;
+  const int esize = kOut == MX_F32 || kOut == MX_F32_ADD ? 4 : 2;
+  p.vec_ok = reinterpret_cast<uintptr_t>(c.C) % (4 * esize) == 0 && c.ldc % 4 == 0;
+  p.status = ctx->d_status;
+  p.debug = ctx->debug_mode;
+  if (c.M <= 16) return launch_narrow<16, kOut>(ctx, c, p, st);
+  if (c.M <= 32) return launch_narrow<32, kOut>(ctx, c, p, st);
+  if (c.M <= 64) return launch_narrow<64, kOut>(ctx, c, p, st);
+  return launch_narrow<128, kOut>(ctx, c, p, st);
+}
+
+}  // namespace
+
+int launch_mx_gemm(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
+  if (c.Cs) return launch_out<MX_MX>(ctx, c, st);
+  switch (c.type) {
+    case AIEHLC_TYPE_F32: return c.accumulate ? launch_out<MX_F32_ADD>(ctx, c, st) : launch_out<MX_F32>(ctx, c, st);
+    case AIEHLC_TYPE_BF16: return launch_out<MX_BF16>(ctx, c, st);
+    default: return launch_out<MX_F16>(ctx, c, st);
+  }
+}
+
+}  // namespace aiehlc

@@ -242,6 +242,14 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -311,6 +319,12 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap,
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
+// Four floats at the shared::cluster address `addr` (mapa_u32).
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 // Barrier arrival (not a data transfer) delivered to the barrier at this offset in every CTA of
 // `cta_mask` once all MMAs issued so far by this thread have retired.
 __device__ __forceinline__ void umma_commit_pair_mask(uint32_t bar, uint16_t cta_mask) {
@@ -351,6 +365,46 @@ __device__ __forceinline__ void umma_ss_i8_halves(uint32_t d_tmem, uint32_t a_lo
       "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
       "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %5, p;\n\t}"
       ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// ------------------------------------------------------------- block-scaled 4-bit products (kind::mxf4)
+// D[tmem] (+)= (A * scaleA) . (B * scaleB): K = 64 e2m1 elements (32 bytes) per instruction, one power-of-two scale per
+// 32 of them.  The scales lie in TMEM: row r of a 128-row operand in lane r % 32 (repeated in every lane quarter),
+// column r / 32, four consecutive K blocks per 32-bit word; the instruction takes two of the four bytes (scale data id
+// 0 or 2 in the instruction descriptor).
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+  if constexpr (kCtaGroup == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
+}
+// 512 bytes of scales (32 lines of 16 bytes) from shared memory to four TMEM columns of every lane quarter; ordered
+// before the products the same thread issues next.  With a CTA pair each CTA's scales go to its own TMEM.
+template <int kCtaGroup>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (kCtaGroup == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Descriptor of such a 512-byte scale tile: no swizzle, groups of eight 16-byte lines 128 bytes apart.
+__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(1) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+// Instruction descriptor of kind::mxf4 (dense, K-major): bits [4,6) scale data id of B, [7,10) and [10,12) e2m1 operands,
+// [17,23) N >> 3, bit 23 power-of-two scales, [27,29) M >> 7, [29,31) scale data id of A.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int scale_id) {
+  return (static_cast<uint32_t>(scale_id) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(scale_id) << 29);
 }
 
 // Instruction descriptor (dense, K-major A and B):

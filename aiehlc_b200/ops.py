@@ -11,6 +11,7 @@ A[M][K] row-major, B stored [N][K], C[M][N] row-major.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 
@@ -58,6 +59,21 @@ def plan_tile_order(M: int, N: int, K: int, kind: str = "int8", num_shards: int 
     if got < 0:
         _capi.check(got)
     return rb[:got], cb[:got], int(slots.value)
+
+
+class MxFp4(NamedTuple):
+    """A microscaled 4-bit matrix [rows][cols]: 32 consecutive elements of a row share a power of two (the format and the
+    layout of the two arrays: aiehlc_b200.h)."""
+    codes: "object"    # uint8 [rows][16 * ceil(cols / 32)]
+    scales: "object"   # uint8 [512 * ceil(rows / 128) * ceil(cols / 128)]
+    rows: int
+    cols: int
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, device) -> "MxFp4":
+        import torch
+        return cls(torch.empty((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=device),
+                   torch.empty(-(-rows // 128) * -(-cols // 128) * 512, dtype=torch.uint8, device=device), rows, cols)
 
 
 class Context:
@@ -332,6 +348,112 @@ class Context:
         _capi.check(self._lib.aiehlc_gemm_bf16_dev(
             self._h, self._dev(A, torch.bfloat16, "A"), self._dev(B, torch.bfloat16, "B"),
             self._dev(out, torch.bfloat16, "C"), M, N, K, self._stream()))
+        return out
+
+    # ------------------------------------------------ microscaled 4-bit matrices
+    def _type(self, dtype, name):
+        import torch
+        try:
+            return {torch.float32: _capi.TYPE_F32, torch.bfloat16: _capi.TYPE_BF16, torch.float16: _capi.TYPE_F16}[dtype]
+        except KeyError:
+            raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {dtype}") from None
+
+    def _rows_of(self, t, name):
+        """(address, type, rows, cols, row pitch) of a matrix whose rows are dense; rows may be further apart."""
+        import torch
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != self.device:
+            raise TypeError(f"{name}: expected a CUDA tensor on device {self.device}")
+        if t.dim() != 2:
+            raise ValueError(f"{name}: expected a matrix")
+        rows, cols = t.shape
+        ld, step = t.stride()
+        if rows <= 1 or cols == 0:
+            ld = cols
+        if (step != 1 and cols > 1) or ld < cols:
+            raise ValueError(f"{name}: the elements of a row must be contiguous and rows must not overlap")
+        return t.data_ptr(), self._type(t.dtype, name), rows, cols, ld
+
+    def _mx(self, q, name):
+        """(codes, scales) addresses of a quantised matrix, with its sizes checked."""
+        if not isinstance(q, MxFp4):
+            raise TypeError(f"{name}: expected an MxFp4")
+        import torch
+        codes, scales, rows, cols = q
+        for t, n, size in ((codes, "codes", rows * (-(-cols // 32) * 16)),
+                           (scales, "scales", -(-rows // 128) * -(-cols // 128) * 512)):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or not t.is_cuda or t.device.index != self.device:
+                raise TypeError(f"{name}.{n}: expected a uint8 CUDA tensor on device {self.device}")
+            if t.numel() != size or not t.is_contiguous():
+                raise ValueError(f"{name}.{n}: expected {size} contiguous bytes for {rows} x {cols}")
+        return codes.data_ptr(), scales.data_ptr()
+
+    def quantize_mxfp4(self, x, way: str = "rows", out=None):
+        """x [rows][cols] (float32, bfloat16 or float16; rows dense, any row pitch) as MxFp4: along its "rows"; along its
+        "columns" (the transposed matrix [cols][rows], its blocks 32 rows of x, which is what products over the rows of x
+        take); or "both", a pair, from one reading."""
+        if way not in ("rows", "columns", "both"):
+            raise ValueError('quantize_mxfp4: way is "rows", "columns" or "both"')
+        addr, kind, rows, cols, ld = self._rows_of(x, "x")
+        q = t = None
+        if out is None:
+            if way != "columns":
+                q = MxFp4.empty(rows, cols, x.device)
+            if way != "rows":
+                t = MxFp4.empty(cols, rows, x.device)
+        else:
+            q, t = out if way == "both" else (out, None) if way == "rows" else (None, out)
+            if (q is not None and (q.rows, q.cols) != (rows, cols)) or (t is not None and (t.rows, t.cols) != (cols, rows)):
+                raise ValueError("quantize_mxfp4: out has other sizes")
+        qc, qs = (None, None) if q is None else self._mx(q, "out")
+        tc, ts = (None, None) if t is None else self._mx(t, "out")
+        _capi.check(self._lib.aiehlc_quantize_mxfp4_dev(self._h, addr, kind, rows, cols, ld, qc, qs, tc, ts, self._stream()))
+        return (q, t) if way == "both" else q if way == "rows" else t
+
+    def dequantize_mxfp4(self, q, dtype=None, out=None):
+        """The values of a quantised matrix (exact in float32 and, the default, bfloat16; float16 rounds)."""
+        import torch
+        codes, scales = self._mx(q, "q")
+        if out is None:
+            out = torch.empty((q.rows, q.cols), dtype=dtype or torch.bfloat16, device=q.codes.device)
+        addr, kind, rows, cols, ld = self._rows_of(out, "out")
+        if (rows, cols) != (q.rows, q.cols) or (dtype is not None and out.dtype != dtype):
+            raise ValueError("dequantize_mxfp4: out has another shape or type")
+        _capi.check(self._lib.aiehlc_dequantize_mxfp4_dev(self._h, codes, scales, rows, cols, addr, kind, ld, self._stream()))
+        return out
+
+    def gemm_mxfp4(self, A, B, dtype=None, out=None, accumulate: bool = False):
+        """C = A . B^T of quantised A [M][K] and B [N][K], sums in 32-bit floating point, in dtype (default bfloat16, or
+        that of `out`).  accumulate: C += A . B^T (float32 only)."""
+        import torch
+        if accumulate and out is None:
+            raise ValueError("gemm_mxfp4: accumulate needs an existing output")
+        ac, as_ = self._mx(A, "A")
+        bc, bs = self._mx(B, "B")
+        if A.cols != B.cols:
+            raise ValueError("gemm_mxfp4: A is [M][K], B is [N][K]; K differs")
+        if out is None:
+            out = torch.empty((A.rows, B.rows), dtype=dtype or torch.bfloat16, device=A.codes.device)
+        addr, kind, M, N, ldc = self._rows_of(out, "out")
+        if (M, N) != (A.rows, B.rows) or (dtype is not None and out.dtype != dtype):
+            raise ValueError("gemm_mxfp4: out has another shape or type")
+        _capi.check(self._lib.aiehlc_gemm_mxfp4_dev(self._h, ac, as_, bc, bs, addr, kind, M, N, A.cols, ldc,
+                                                    1 if accumulate else 0, self._stream()))
+        return out
+
+    def gemm_mxfp4_mxfp4(self, A, B, out=None):
+        """The same product quantised again by its output stage, from the 32-bit sums: an MxFp4 [M][N], the operand of
+        the next product in a chain."""
+        ac, as_ = self._mx(A, "A")
+        bc, bs = self._mx(B, "B")
+        if A.cols != B.cols:
+            raise ValueError("gemm_mxfp4_mxfp4: A is [M][K], B is [N][K]; K differs")
+        if out is None:
+            out = MxFp4.empty(A.rows, B.rows, A.codes.device)
+        elif (out.rows, out.cols) != (A.rows, B.rows):
+            raise ValueError("gemm_mxfp4_mxfp4: out has other sizes")
+        cc, cs = self._mx(out, "out")
+        _capi.check(self._lib.aiehlc_gemm_mxfp4_mxfp4_dev(self._h, ac, as_, bc, bs, cc, cs, A.rows, B.rows, A.cols,
+                                                          self._stream()))
         return out
 
     def conv2d_i8_srs(self, x, w, shift_vec, pad: int = 1, out=None):

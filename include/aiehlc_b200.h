@@ -119,6 +119,47 @@ int aiehlc_gemm_bf16_dev(aiehlc_ctx* ctx, const uint16_t* A, const uint16_t* B, 
 int aiehlc_gemm_bf16_host(aiehlc_ctx* ctx, const uint16_t* A, const uint16_t* B, uint16_t* C, int M,
                           int N, int K);
 
+/* ---- microscaled 4-bit matrices (MXFP4 of the OCP Microscaling specification) --------------
+ * A block is 32 consecutive elements of a row (the last block of a row may be shorter).  It shares a power of
+ * two 2^e and holds e2m1 numbers: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+ *     e     = floor(log2(max |x|)) - 2, at least -127
+ *     value = 2^e * e2m1(x / 2^e)          nearest, ties to even, at most 6 * 2^e in magnitude
+ * A block with an infinity or a NaN in it becomes NaN as a whole.
+ * A quantised matrix of `rows` x `cols` is two dense arrays, both 16-byte aligned:
+ *     codes   [rows][aiehlc_mxfp4_pitch(cols)]     element 2i in the low half of byte i; zeros past column cols - 1
+ *     scales  aiehlc_mxfp4_scale_bytes(rows, cols) bytes, e + 127 (255: NaN), in tiles of 128 rows x 4 blocks: row r,
+ *             block b at ((r / 128) * ceil(blocks / 4) + b / 4) * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4;
+ *             zeros for rows and blocks of a tile that do not exist
+ * Operands that the caller lays out keep the zeros too: a padding block with scale 255 would make its row NaN.
+ * None of these calls uses a workspace: calls on different streams and captured graphs may overlap as long as their
+ * own buffers do not.  No counterpart in the reference (its kernels are integer). */
+#define AIEHLC_TYPE_F32 0
+#define AIEHLC_TYPE_BF16 1
+#define AIEHLC_TYPE_F16 2
+long long aiehlc_mxfp4_pitch(long long cols);                        /* 16 * ceil(cols / 32) */
+long long aiehlc_mxfp4_scale_bytes(long long rows, long long cols);  /* 512 * ceil(rows / 128) * ceil(cols / 128) */
+/* x [rows][cols] of `type`, row pitch `ld` elements (>= cols), quantised from one reading
+ *   along its rows into q, q_scales                  (NULL, NULL: not wanted)
+ *   along its columns into t, t_scales, as the transposed matrix [cols][rows] with blocks of 32 rows of x
+ *                                                    (NULL, NULL: not wanted)
+ * The second is what a product over the rows of x takes: gradients by weights and by activations. */
+int aiehlc_quantize_mxfp4_dev(aiehlc_ctx* ctx, const void* x, int type, long long rows, long long cols, long long ld,
+                              uint8_t* q, uint8_t* q_scales, uint8_t* t, uint8_t* t_scales, void* stream);
+/* The values of a quantised matrix, y [rows][cols] of `type`, row pitch `ld` elements.  Exact in f32 and bf16; f16
+ * rounds to nearest even and overflows to infinity. */
+int aiehlc_dequantize_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* q, const uint8_t* q_scales, long long rows, long long cols,
+                                void* y, int type, long long ld, void* stream);
+/* C[i][j] = sum_k A[i][k] * B[j][k] of quantised A [M][K] and B [N][K], sums in 32-bit floating point, C of `type` with row
+ * pitch `ldc` elements (>= N), rounded once.  accumulate != 0 (type AIEHLC_TYPE_F32 only): C += A.B^T.
+ * M, N, K up to 2^30. */
+int aiehlc_gemm_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* A, const uint8_t* A_scales, const uint8_t* B,
+                          const uint8_t* B_scales, void* C, int type, int M, int N, int K, long long ldc, int accumulate,
+                          void* stream);
+/* The same product with a quantising output stage: C [M][N] as codes and scales, blocks along its rows, from the 32-bit
+ * sums -- the operand of the next product in a chain. */
+int aiehlc_gemm_mxfp4_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* A, const uint8_t* A_scales, const uint8_t* B,
+                                const uint8_t* B_scales, uint8_t* C, uint8_t* C_scales, int M, int N, int K, void* stream);
+
 /* ---- int8 conv2d as an implicit GEMM, per-output-channel srs ------------------------------
  * x: NHWC int8 [n][h][w][cin]; w: HWIO int8 [kh][kw][cin][cout]; y: NHWC int8 [n][h][w][cout]
  * stride 1, zero padding `pad` on every side, output spatial size = input spatial size

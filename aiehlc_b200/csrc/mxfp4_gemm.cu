@@ -27,6 +27,8 @@ struct MxGemmParams {
   long long ldc;
   int vec_ok;               // four results at a time may be stored as a vector
   int m_tiles, n_tiles;
+  int group_m;              // CTA pairs: row blocks walked before the next column block
+  int tile_store;           // CTA pairs: results leave as TMA tile stores
   int* status;
   int debug;                // 3: the producer withholds its loads, so every wait runs out
 };
@@ -45,8 +47,8 @@ struct NarrowShape {
   static constexpr int kPartialBytes = kTN * 128 * 4;         // over the stages, once they are done
   static constexpr int kPool = kStages * kStageBytes > kPartialBytes ? kStages * kStageBytes : kPartialBytes;
   static constexpr int kTotal = 1024 + kPool + 256;
-  static constexpr int kScaleCols = 32;                       // two sets of 8 columns for each operand
-  static constexpr int kTmemCols = kTN <= 32 ? 64 : kTN == 64 ? 128 : 256;
+  static constexpr int kScaleCols = 16 * kStages;             // per stage 8 columns of each operand's scales
+  static constexpr int kTmemCols = kTN <= 64 ? 128 : 256;
   static_assert(kTN + kScaleCols <= kTmemCols, "TMEM");
 };
 
@@ -193,7 +195,7 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       tc_fence_after();
       const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
       const uint32_t scales = at + S::kBBytes + S::kABytes;
-      const uint32_t t_scales = tmem_base + kTN + (k & 1) * 16;  // 8 columns of B's scales, 8 of A's
+      const uint32_t t_scales = tmem_base + kTN + stage * 16;  // 8 columns of B's scales, 8 of A's; free like the stage
       const int mmas = min(kStepK, p.K - k * kStepK + kMmaK - 1) / kMmaK;
 #pragma unroll
       for (int w = 0; w < 2; ++w)
@@ -263,6 +265,14 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   }
 }
 
+}  // namespace
+}  // namespace aiehlc
+
+#include "mxfp4_gemm_pair.cuh"
+
+namespace aiehlc {
+namespace {
+
 int encode_codes_map(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* codes, long long rows, long long cols, int box_rows) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(mx_pitch(cols)), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(mx_pitch(cols))};
@@ -308,6 +318,99 @@ int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStr
   return AIEHLC_OK;
 }
 
+// Codes as a 3-D tensor {128 bytes, rows, K / 256}: one box brings `steps` steps of K.  K a multiple of 256.
+int encode_codes_map_3d(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* codes, long long rows, long long cols, int box_rows, int steps) {
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(cols / kStepK)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(mx_pitch(cols)), 128};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(steps)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(codes), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AIEHLC_ERR_CUDA, "cuTensorMapEncodeTiled (3-D) failed for the codes of a 4-bit operand");
+  return AIEHLC_OK;
+}
+
+// Scales as a matrix with one row per 128 rows of the operand, in 8-byte elements; a box brings `steps` steps of K of
+// `box_rows` such rows.  What lies outside reads as zero.
+int encode_scales_map(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* scales, long long rows, long long cols, int box_rows, int steps) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(mx_words(cols) * (kMxScaleTile / 8)), static_cast<cuuint64_t>((rows + 127) / 128)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(mx_words(cols) * kMxScaleTile)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(steps * kStepScales / 8), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<uint8_t*>(scales), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AIEHLC_ERR_CUDA, "cuTensorMapEncodeTiled failed for the scales of a 4-bit operand");
+  return AIEHLC_OK;
+}
+
+// C as the output warps store it: 32 rows x 128 bytes (codes of a kBN-column tile: kBN / 2 bytes).
+template <int kBN, int kOut>
+int encode_result_map(aiehlc_ctx* ctx, CUtensorMap* map, const MxGemmCall& c) {
+  constexpr int esize = kOut == MX_MX ? 1 : kOut == MX_F32 || kOut == MX_F32_ADD ? 4 : 2;
+  constexpr int row_bytes = kOut == MX_MX ? kBN / 2 : 128;
+  const long long cols = kOut == MX_MX ? mx_pitch(c.N) : c.N;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(c.M)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(kOut == MX_MX ? cols : c.ldc * esize)};
+  const cuuint32_t box[2] = {row_bytes / esize, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = kOut == MX_MX ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : kOut == MX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : kOut == MX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const CUresult r = ctx->encode(map, type, 2, c.C, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AIEHLC_ERR_CUDA, "cuTensorMapEncodeTiled failed for the result of a 4-bit product");
+  return AIEHLC_OK;
+}
+
+template <int kBN, int kKPer, int kOut>
+int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStream_t st) {
+  using S = MxPairShape<kBN, kKPer>;
+  CUtensorMap ma, mb, mas, mbs, mc;
+  if constexpr (kKPer == 1) {
+    if (int rc = encode_codes_map(ctx, &ma, c.A, c.M, c.K, 128)) return rc;
+    if (int rc = encode_codes_map(ctx, &mb, c.B, c.N, c.K, kBN / 2)) return rc;
+  } else {
+    if (int rc = encode_codes_map_3d(ctx, &ma, c.A, c.M, c.K, 128, kKPer)) return rc;
+    if (int rc = encode_codes_map_3d(ctx, &mb, c.B, c.N, c.K, kBN / 2, kKPer)) return rc;
+  }
+  if (int rc = encode_scales_map(ctx, &mas, c.As, c.M, c.K, 1, kKPer)) return rc;
+  if (int rc = encode_scales_map(ctx, &mbs, c.Bs, c.N, c.K, S::kBTiles, kKPer)) return rc;
+  constexpr int esize = kOut == MX_F32 || kOut == MX_F32_ADD ? 4 : 2;
+  // a tile store is clipped at the tensor's edge in pieces of 16 bytes: a row that ends inside one would be written past its end
+  p.tile_store = kOut == MX_MX || (kOut != MX_F32_ADD && reinterpret_cast<uintptr_t>(c.C) % 16 == 0 && c.ldc * esize % 16 == 0 &&
+                                   static_cast<long long>(c.N) * esize % 16 == 0);
+  mc = ma;  // unused without tile stores
+  if (p.tile_store)
+    if (int rc = encode_result_map<kBN, kOut>(ctx, &mc, c)) return rc;
+  p.m_tiles = (c.M + 255) / 256;
+  p.n_tiles = (c.N + kBN - 1) / kBN;
+  p.group_m = ctx->group_m > 0 ? ctx->group_m : 8;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  auto kern = mx_gemm_pair_kernel<kBN, kKPer, kOut>;
+  KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
+  if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::kTotal, &ks.smem_attr)) return rc;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  const long long limit = ctx->usable_sms() / 2 > 0 ? ctx->usable_sms() / 2 : 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < limit ? tiles : limit)));
+  cfg.blockDim = dim3(kMxPairThreads);
+  cfg.dynamicSmemBytes = S::kTotal;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctx->pdl ? 2 : 1;
+  AIEHLC_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, mas, mbs, mc, p));
+  ctx->launches++;
+  return AIEHLC_OK;
+}
+
 template <int kOut>
 int launch_out(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
   MxGemmParams p{};
@@ -320,6 +423,13 @@ int launch_out(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
   p.vec_ok = reinterpret_cast<uintptr_t>(c.C) % (4 * esize) == 0 && c.ldc % 4 == 0;
   p.status = ctx->d_status;
   p.debug = ctx->debug_mode;
+  if (c.M > 128 || ctx->pair_mode == 1) {
+    const bool two = c.K % kStepK == 0 && c.K >= 2 * kStepK && ctx->k_per_load != 1;
+    const long long tiles = ((c.M + 255LL) / 256) * ((c.N + 255LL) / 256);
+    if (ctx->force_tile_n == 128 || (ctx->force_tile_n == 0 && tiles * 2 <= ctx->usable_sms() / 2))
+      return two ? launch_pair<128, 2, kOut>(ctx, c, p, st) : launch_pair<128, 1, kOut>(ctx, c, p, st);
+    return two ? launch_pair<256, 2, kOut>(ctx, c, p, st) : launch_pair<256, 1, kOut>(ctx, c, p, st);
+  }
   if (c.M <= 16) return launch_narrow<16, kOut>(ctx, c, p, st);
   if (c.M <= 32) return launch_narrow<32, kOut>(ctx, c, p, st);
   if (c.M <= 64) return launch_narrow<64, kOut>(ctx, c, p, st);

@@ -1,0 +1,365 @@
+// Products of microscaled 4-bit matrices by CTA pairs (tcgen05 cta_group::2): two CTAs on neighbouring SMs share one
+// 256 x kBN tile of C, persistent over the tiles.  Included by mxfp4_gemm.cu.
+//
+//   warp 0 (both CTAs)  fetches this CTA's 128 rows of A, its half of B's rows, the scales of its A rows and the scales of
+//                       all of the tile's B rows (each CTA multiplies with all of B); everything is credited to the
+//                       leader's "full" barrier
+//   warp 1 (leader)     copies the scales to TMEM and issues the products, M = 256, K = 64 each
+//   warps 2-5           drain this CTA's 128 accumulator rows through the output stage
+//
+// TMEM (512 columns per CTA): two accumulators of kBN columns and two sets of scales of 24 columns (256 elements of K:
+// two words, 4 columns of A's and up to 8 of B's each).  With kBN = 256 the accumulators share 48 columns, which makes the
+// room for the scales: accumulator 0 takes columns 0-255, accumulator 1 columns 208-463.  The output stage reads
+// the 64 columns that hold the shared ones first and hands them back at once, so that the next tile's products wait for
+// one TMEM read, not for the whole output stage.
+#pragma once
+
+namespace aiehlc {
+
+namespace {
+
+constexpr int kMxPairThreads = 192;
+
+template <int kBN, int kKPer>
+struct MxPairShape {
+  static constexpr int kABlock = 128 * 128;                    // 256 elements of K of this CTA's rows of A
+  static constexpr int kBBlock = kBN / 2 * 128;
+  static constexpr int kBTiles = kBN / 128;                    // scale tiles (of 128 rows) across the tile's columns
+  static constexpr int kABytes = kABlock * kKPer;
+  static constexpr int kBBytes = kBBlock * kKPer;
+  static constexpr int kAScales = kStepScales * kKPer;
+  static constexpr int kBScales = kStepScales * kKPer * kBTiles;
+  static constexpr int kStageBytes = kABytes + kBBytes + kAScales + kBScales;
+  static constexpr int kStagingBytes = 4 * 4096;               // one buffer of 32 rows x 128 bytes per output warp
+  static constexpr int kBarBytes = 1024;
+  static constexpr int kLimit = 227 * 1024;
+  static constexpr int kStages = (kLimit - kStagingBytes - kBarBytes) / kStageBytes > 8 ? 8 : (kLimit - kStagingBytes - kBarBytes) / kStageBytes;
+  static constexpr int kTotal = kStages * kStageBytes + kStagingBytes + kBarBytes;
+  static constexpr bool kShared = kBN == 256;
+  static constexpr int kAcc1 = kBN == 256 ? 208 : kBN;         // first column of accumulator 1
+  static constexpr int kScaleCol = kBN == 256 ? 464 : 2 * kBN;
+  static constexpr int kTmemCols = 512;
+  static_assert(kStageBytes % 1024 == 0 && kScaleCol + 48 <= kTmemCols, "layout");
+};
+
+// Tiles walk group_m row blocks before the next column block.
+__device__ __forceinline__ void mx_tile(const MxGemmParams& p, int t, int& mb, int& nb) {
+  const int per_group = p.group_m * p.n_tiles;
+  const int g = t / per_group;
+  const int first = g * p.group_m;
+  const int rows = min(p.group_m, p.m_tiles - first);
+  const int r = t - g * per_group;
+  mb = first + r % rows;
+  nb = r / rows;
+}
+
+// 32 rows x 32 columns of C, one row per lane, through this warp's staging buffer: out in whole 128-byte (f32) or
+// 64-byte row pieces, where C does not allow tile stores or is added to.
+template <int kOut>
+__device__ __forceinline__ void store_rows(const MxGemmParams& p, uint8_t* buf, const uint32_t (&r)[32], int row0, int col0, int lane) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+  __syncwarp();
+  const int piece = lane & 7;
+  const int n = col0 + piece * 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int at = i * 4 + (lane >> 3);
+    const float4 v = *reinterpret_cast<const float4*>(buf + at * 128 + ((piece ^ (at & 7)) << 4));
+    if (row0 + at < p.M && n < p.N) store4<kOut>(p, row0 + at, n, v);
+  }
+  __syncwarp();
+}
+
+template <int kBN, int kKPer, int kOut>
+__global__ void __launch_bounds__(kMxPairThreads, 1)
+mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                    const __grid_constant__ CUtensorMap tmap_as, const __grid_constant__ CUtensorMap tmap_bs,
+                    const __grid_constant__ CUtensorMap tmap_c, const MxGemmParams p) {
+  using S = MxPairShape<kBN, kKPer>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];   // nothing static: the dynamic part starts on its 1024-byte boundary
+  uint8_t* staging = smem + kStages * S::kStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + S::kStagingBytes);  // used in the leader
+  uint64_t* empty_bar = full_bar + kStages;           // one set per CTA
+  uint64_t* scale_bar = empty_bar + kStages;          // used in the leader: the products that read a set of scales are done
+  uint64_t* tmem_full_bar = scale_bar + 2;            // one set per CTA
+  uint64_t* tmem_free_bar = tmem_full_bar + 2;        // used in the leader: one per accumulator, or one for what they share
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_free_bar + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = rank == 0;
+  const int pair_id = static_cast<int>(cluster_id_x());
+  const int num_pairs = static_cast<int>(cluster_count_x());
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&scale_bar[a]), 1);
+      mbar_init(smem_u32(&tmem_full_bar[a]), 1);
+      mbar_init(smem_u32(&tmem_free_bar[a]), 8);      // every output warp of the two CTAs
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_as);
+    tma_prefetch_desc(&tmap_bs);
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(smem_u32(tmem_base_slot), S::kTmemCols);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int num_tiles = p.m_tiles * p.n_tiles;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair_id; ok && t < num_tiles; t += num_pairs) {
+        int mb, nb;
+        mx_tile(p, t, mb, nb);
+        for (int k = 0; k < p.k_steps; k += kKPer) {
+          ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status, ST_TIMEOUT_EMPTY);
+          if (!ok) break;
+          if (p.debug != 3) {
+            if (leader) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * S::kStageBytes);
+            const uint32_t bar = mapa_u32(smem_u32(&full_bar[stage]), 0);
+            const uint32_t sa = smem_u32(smem + stage * S::kStageBytes);
+            const uint32_t sb = sa + S::kABytes;
+            const uint32_t ss = sb + S::kBBytes;
+            const int row_a = mb * 256 + rank * 128;
+            const int row_b = nb * kBN + rank * (kBN / 2);
+            if constexpr (kKPer == 1) {
+              tma_load_2d_pair(sa, &tmap_a, bar, k * 128, row_a);
+              tma_load_2d_pair(sb, &tmap_b, bar, k * 128, row_b);
+            } else {
+              tma_load_3d_pair(sa, &tmap_a, bar, 0, row_a, k);   // steps past the end of K read as zero
+              tma_load_3d_pair(sb, &tmap_b, bar, 0, row_b, k);
+            }
+            tma_load_2d_pair(ss, &tmap_as, bar, k * (kStepScales / 8), mb * 2 + rank);
+            tma_load_2d_pair(ss + S::kAScales, &tmap_bs, bar, k * (kStepScales / 8), nb * S::kBTiles);
+          }
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok)
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land before the CTA retires
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t sets = 0;                              // sets of scales used so far
+      int it = 0;
+      bool ok = true;
+      for (int t = pair_id; ok && t < num_tiles; t += num_pairs, ++it) {
+        // The output stage has drained the accumulator's tile before this one.  Where the accumulators share columns, what
+        // it signals is that it has read the shared ones of the last tile, for which it was through with the tile before.
+        if constexpr (S::kShared) ok = it == 0 || mbar_wait(smem_u32(tmem_free_bar), (it - 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
+        else ok = it < 2 || mbar_wait(smem_u32(&tmem_free_bar[it & 1]), ((it >> 1) - 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (it & 1) * S::kAcc1;
+        for (int k = 0; k < p.k_steps; k += kKPer) {
+          ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * S::kStageBytes);
+          const uint32_t sb = sa + S::kABytes;
+          const uint32_t ss = sb + S::kBBytes;
+#pragma unroll
+          for (int kk = 0; kk < kKPer; ++kk) {
+            if (k + kk >= p.k_steps) break;
+            const int mmas = min(kStepK, p.K - (k + kk) * kStepK + kMmaK - 1) / kMmaK;
+            // the set's last readers (two steps ago) are done; the step before keeps the tensor cores busy meanwhile
+            if (sets >= 2) {
+              ok = mbar_wait(smem_u32(&scale_bar[sets & 1]), ((sets >> 1) - 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
+              if (!ok) break;
+            }
+            const uint32_t t_scales = tmem_base + S::kScaleCol + (sets & 1) * 24;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              if (2 * w < mmas) {
+                tmem_copy_scales<2>(t_scales + w * 12, make_scale_desc(ss + (2 * kk + w) * kMxScaleTile));
+#pragma unroll
+                for (int b = 0; b < S::kBTiles; ++b)
+                  tmem_copy_scales<2>(t_scales + w * 12 + 4 + 4 * b,
+                                      make_scale_desc(ss + S::kAScales + (b * 2 * kKPer + 2 * kk + w) * kMxScaleTile));
+              }
+            }
+            const uint64_t adesc = make_kmajor_desc(sa + kk * S::kABlock, 1024, 2);
+            const uint64_t bdesc = make_kmajor_desc(sb + kk * S::kBBlock, 1024, 2);
+#pragma unroll
+            for (int i = 0; i < kStepK / kMmaK; ++i)
+              if (i < mmas)
+                umma_mxf4<2>(d_tmem, adesc + 2 * i, bdesc + 2 * i, make_idesc_mxf4(256, kBN, 2 * (i & 1)),
+                             t_scales + (i >> 1) * 12, t_scales + (i >> 1) * 12 + 4, (k + kk > 0 || i > 0) ? 1u : 0u);
+            umma_commit_pair_mask(smem_u32(&scale_bar[sets & 1]), 1);
+            ++sets;
+          }
+          if (!ok) break;
+          umma_commit_pair_mask(smem_u32(&empty_bar[stage]), 3);
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma_commit_pair_mask(smem_u32(&tmem_full_bar[it & 1]), 3);
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    uint8_t* buf = staging + quad * 4096;
+    const int swz = lane & 7;
+    int it = 0;
+    for (int t = pair_id; t < num_tiles; t += num_pairs, ++it) {
+      int mb, nb;
+      mx_tile(p, t, mb, nb);
+      const int acc = it & 1;
+      bool ok = mbar_wait(smem_u32(&tmem_full_bar[acc]), (it >> 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const int row0 = mb * 256 + rank * 128 + quad * 32;
+      const int n0 = nb * kBN;
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::kAcc1;
+      uint32_t words[kBN / 128] = {};                  // MX_MX: this row's scales
+#pragma unroll 1
+      for (int step = 0; step < kBN / 64; ++step) {
+        // accumulator 0 of 256 columns shares its last ones, accumulator 1 its first
+        const int c = S::kShared && acc == 0 ? (step == 0 ? 192 : 64 * (step - 1)) : 64 * step;
+        uint32_t r[2][32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(taddr + c, r[0]);
+        tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
+        tmem_ld_wait();
+        if (step == (S::kShared ? 0 : kBN / 64 - 1)) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(smem_u32(&tmem_free_bar[S::kShared ? 0 : acc]), 0);
+        }
+        if constexpr (kOut == MX_MX) {
+          if (step == 0) {
+            if (lane == 0) tma_store_wait_read<0>();   // the tile before has left the buffer
+            __syncwarp();
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int n = n0 + c + 32 * h;
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (n + j >= p.N) r[h][j] = 0;
+              most = max(most, r[h][j] & 0x7FFFFFFFu);
+            }
+            const int s = mx_scale_of(most);
+            const float inv = mx_inverse(s);
+            uint32_t w[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              float f[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) f[j] = mx_scaled(__uint_as_float(r[h][8 * g + j]), inv);
+              w[g] = mx_codes8(f);
+            }
+            const int piece = c / 32 + h;              // 16 bytes of codes per block
+            *reinterpret_cast<uint4*>(buf + lane * (kBN / 2) + ((piece ^ (kBN == 256 ? swz : (lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            const uint32_t byte = row0 + lane < p.M && n < p.N ? static_cast<uint32_t>(s) << (8 * (piece & 3)) : 0u;
+            if (kBN == 256 && piece >= 4) words[kBN / 128 - 1] |= byte;
+            else words[0] |= byte;
+          }
+        } else if (kOut != MX_F32_ADD && p.tile_store) {
+          if constexpr (kOut == MX_F32) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (lane == 0) tma_store_wait_read<0>();
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ swz) << 4)) = make_uint4(r[h][4 * j], r[h][4 * j + 1], r[h][4 * j + 2], r[h][4 * j + 3]);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&tmap_c, smem_u32(buf), n0 + c + 32 * h, row0);
+                tma_store_commit();
+              }
+            }
+          } else {
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float lo = __uint_as_float(r[j >> 2][8 * (j & 3) + 2 * i]), hi = __uint_as_float(r[j >> 2][8 * (j & 3) + 2 * i + 1]);
+                if constexpr (kOut == MX_BF16) {
+                  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+                  w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                } else {
+                  const __half2 v = __floats2half2_rn(lo, hi);
+                  w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+              }
+              *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ swz) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmap_c, smem_u32(buf), n0 + c, row0);
+              tma_store_commit();
+            }
+          }
+        } else {
+          store_rows<kOut>(p, buf, r[0], row0, n0 + c, lane);
+          store_rows<kOut>(p, buf, r[1], row0, n0 + c + 32, lane);
+        }
+      }
+      if constexpr (kOut == MX_MX) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tmap_c, smem_u32(buf), n0 / 2, row0);
+          tma_store_commit();
+        }
+        // scale words of this row; rows past M are zeros up to the end of their scale tile
+        const long long c_words = mx_words(p.N);
+        if (row0 / 128 < (p.M + 127) / 128) {
+#pragma unroll
+          for (int w = 0; w < kBN / 128; ++w)
+            if (n0 / 128 + w < c_words)
+              *reinterpret_cast<uint32_t*>(p.c_scales + (static_cast<long long>(row0 / 128) * c_words + n0 / 128 + w) * kMxScaleTile +
+                                           mx_scale_word((row0 + lane) & 127)) = words[w];
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait_all();
+  }
+
+  // Neither CTA retires or frees TMEM while its partner can still read its shared memory or signal its barriers.
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem_base, S::kTmemCols);
+  }
+}
+
+}  // namespace
+
+}  // namespace aiehlc

@@ -1,24 +1,30 @@
 // Products of microscaled 4-bit matrices by CTA pairs (tcgen05 cta_group::2): two CTAs on neighbouring SMs share one
 // 256 x kBN tile of C, persistent over the tiles.  Included by mxfp4_gemm.cu.
 //
-//   warp 0 (both CTAs)  fetches this CTA's 128 rows of A, its half of B's rows, the scales of its A rows and the scales of
-//                       all of the tile's B rows (each CTA multiplies with all of B); everything is credited to the
-//                       leader's "full" barrier
-//   warp 1 (leader)     copies the scales to TMEM and issues the products, M = 256, K = 64 each
+//   warp 0 (both CTAs)  fetches this CTA's 128 rows of A and its half of B's rows (credited to the leader's "full"
+//                       barrier), the scales of its A rows and those of all of the tile's B rows (each CTA multiplies with
+//                       all of B; credited to its own "scales full" barrier)
+//   warp 1 (leader)     issues the products, M = 256, K = 64 each
 //   warps 2-5           drain this CTA's 128 accumulator rows through the output stage
+//   warps 6-9           move the scales from shared memory to this CTA's TMEM, one lane quarter each
 //
-// TMEM (512 columns per CTA): two accumulators of kBN columns and two sets of scales of 24 columns (256 elements of K:
-// two words, 4 columns of A's and up to 8 of B's each).  With kBN = 256 the accumulators share 48 columns, which makes the
-// room for the scales: accumulator 0 takes columns 0-255, accumulator 1 columns 208-463.  The output stage reads
-// the 64 columns that hold the shared ones first and hands them back at once, so that the next tile's products wait for
-// one TMEM read, not for the whole output stage.
+// Why warps and not tcgen05.cp: the copies run in the tensor cores' own queue, between the products, not beside them.  Measured
+// on 512 x 9472 x 65536 (one tile per pair): 166 cycles per product without copies, 240 with six 512-byte copies per four
+// products (about 30 cycles a copy and 64 each time the queue turns from products to copies), 313 with the
+// commits that tell when a set of scales may be overwritten.
+//
+// TMEM (512 columns per CTA): two accumulators of kBN columns and kSets sets of scales, one per stage in flight: for each
+// 128 elements of K, 4 columns of A's scales and kBN / 32 of B's.  With kBN = 256 the accumulators share 96 columns, which
+// makes the room: accumulator 0 takes columns 0-255, accumulator 1 columns 160-415.  The output stage reads the
+// half of a tile that holds the shared columns first and hands them back at once, so that the next tile's products
+// wait for one read of TMEM, not for the whole output stage.
 #pragma once
 
 namespace aiehlc {
 
 namespace {
 
-constexpr int kMxPairThreads = 192;
+constexpr int kMxPairThreads = 320;
 
 template <int kBN, int kKPer>
 struct MxPairShape {
@@ -36,10 +42,13 @@ struct MxPairShape {
   static constexpr int kStages = (kLimit - kStagingBytes - kBarBytes) / kStageBytes > 8 ? 8 : (kLimit - kStagingBytes - kBarBytes) / kStageBytes;
   static constexpr int kTotal = kStages * kStageBytes + kStagingBytes + kBarBytes;
   static constexpr bool kShared = kBN == 256;
-  static constexpr int kAcc1 = kBN == 256 ? 208 : kBN;         // first column of accumulator 1
-  static constexpr int kScaleCol = kBN == 256 ? 464 : 2 * kBN;
+  static constexpr int kAcc1 = kBN == 256 ? 160 : kBN;         // first column of accumulator 1
+  static constexpr int kWordCols = 4 + 4 * kBTiles;            // columns of scales per 128 elements of K
+  static constexpr int kSetCols = 2 * kKPer * kWordCols;
+  static constexpr int kSets = 4 / kKPer;
+  static constexpr int kScaleCol = kAcc1 + kBN;
   static constexpr int kTmemCols = 512;
-  static_assert(kStageBytes % 1024 == 0 && kScaleCol + 48 <= kTmemCols, "layout");
+  static_assert(kStageBytes % 1024 == 0 && kScaleCol + kSets * kSetCols <= kTmemCols && kSets <= kStages, "layout");
 };
 
 // Tiles walk group_m row blocks before the next column block.
@@ -83,8 +92,9 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   uint8_t* staging = smem + kStages * S::kStageBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + S::kStagingBytes);  // used in the leader
   uint64_t* empty_bar = full_bar + kStages;           // one set per CTA
-  uint64_t* scale_bar = empty_bar + kStages;          // used in the leader: the products that read a set of scales are done
-  uint64_t* tmem_full_bar = scale_bar + 2;            // one set per CTA
+  uint64_t* scales_full_bar = empty_bar + kStages;    // one set per CTA
+  uint64_t* scales_set_bar = scales_full_bar + kStages;  // used in the leader: a set of scales is in TMEM
+  uint64_t* tmem_full_bar = scales_set_bar + S::kSets;   // one set per CTA
   uint64_t* tmem_free_bar = tmem_full_bar + 2;        // used in the leader: one per accumulator, or one for what they share
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_free_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
@@ -100,9 +110,10 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
+      mbar_init(smem_u32(&scales_full_bar[s]), 1);
     }
+    for (int a = 0; a < S::kSets; ++a) mbar_init(smem_u32(&scales_set_bar[a]), 8);  // the scale warps of the two CTAs
     for (int a = 0; a < 2; ++a) {
-      mbar_init(smem_u32(&scale_bar[a]), 1);
       mbar_init(smem_u32(&tmem_full_bar[a]), 1);
       mbar_init(smem_u32(&tmem_free_bar[a]), 8);      // every output warp of the two CTAs
     }
@@ -139,7 +150,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status, ST_TIMEOUT_EMPTY);
           if (!ok) break;
           if (p.debug != 3) {
-            if (leader) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * S::kStageBytes);
+            if (leader) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * (S::kABytes + S::kBBytes));
             const uint32_t bar = mapa_u32(smem_u32(&full_bar[stage]), 0);
             const uint32_t sa = smem_u32(smem + stage * S::kStageBytes);
             const uint32_t sb = sa + S::kABytes;
@@ -153,8 +164,10 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
               tma_load_3d_pair(sa, &tmap_a, bar, 0, row_a, k);   // steps past the end of K read as zero
               tma_load_3d_pair(sb, &tmap_b, bar, 0, row_b, k);
             }
-            tma_load_2d_pair(ss, &tmap_as, bar, k * (kStepScales / 8), mb * 2 + rank);
-            tma_load_2d_pair(ss + S::kAScales, &tmap_bs, bar, k * (kStepScales / 8), nb * S::kBTiles);
+            const uint32_t scales_bar = smem_u32(&scales_full_bar[stage]);
+            mbar_expect_tx(scales_bar, S::kAScales + S::kBScales);
+            tma_load_2d(ss, &tmap_as, scales_bar, k * (kStepScales / 8), mb * 2 + rank);
+            tma_load_2d(ss + S::kAScales, &tmap_bs, scales_bar, k * (kStepScales / 8), nb * S::kBTiles);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
@@ -166,7 +179,8 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     if (lane == 0 && leader) {
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t sets = 0;                              // sets of scales used so far
+      int set = 0;
+      uint32_t set_phase = 0;
       int it = 0;
       bool ok = true;
       for (int t = pair_id; ok && t < num_tiles; t += num_pairs, ++it) {
@@ -181,44 +195,71 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL);
           if (!ok) break;
           tc_fence_after();
+          ok = mbar_wait(smem_u32(&scales_set_bar[set]), set_phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+          if (!ok) break;
+          tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * S::kStageBytes);
           const uint32_t sb = sa + S::kABytes;
-          const uint32_t ss = sb + S::kBBytes;
+          const uint32_t t_scales = tmem_base + S::kScaleCol + set * S::kSetCols;
 #pragma unroll
           for (int kk = 0; kk < kKPer; ++kk) {
             if (k + kk >= p.k_steps) break;
             const int mmas = min(kStepK, p.K - (k + kk) * kStepK + kMmaK - 1) / kMmaK;
-            // the set's last readers (two steps ago) are done; the step before keeps the tensor cores busy meanwhile
-            if (sets >= 2) {
-              ok = mbar_wait(smem_u32(&scale_bar[sets & 1]), ((sets >> 1) - 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
-              if (!ok) break;
-            }
-            const uint32_t t_scales = tmem_base + S::kScaleCol + (sets & 1) * 24;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              if (2 * w < mmas) {
-                tmem_copy_scales<2>(t_scales + w * 12, make_scale_desc(ss + (2 * kk + w) * kMxScaleTile));
-#pragma unroll
-                for (int b = 0; b < S::kBTiles; ++b)
-                  tmem_copy_scales<2>(t_scales + w * 12 + 4 + 4 * b,
-                                      make_scale_desc(ss + S::kAScales + (b * 2 * kKPer + 2 * kk + w) * kMxScaleTile));
-              }
-            }
             const uint64_t adesc = make_kmajor_desc(sa + kk * S::kABlock, 1024, 2);
             const uint64_t bdesc = make_kmajor_desc(sb + kk * S::kBBlock, 1024, 2);
 #pragma unroll
-            for (int i = 0; i < kStepK / kMmaK; ++i)
+            for (int i = 0; i < kStepK / kMmaK; ++i) {
+              const uint32_t t_word = t_scales + (2 * kk + (i >> 1)) * S::kWordCols;
               if (i < mmas)
-                umma_mxf4<2>(d_tmem, adesc + 2 * i, bdesc + 2 * i, make_idesc_mxf4(256, kBN, 2 * (i & 1)),
-                             t_scales + (i >> 1) * 12, t_scales + (i >> 1) * 12 + 4, (k + kk > 0 || i > 0) ? 1u : 0u);
-            umma_commit_pair_mask(smem_u32(&scale_bar[sets & 1]), 1);
-            ++sets;
+                umma_mxf4<2>(d_tmem, adesc + 2 * i, bdesc + 2 * i, make_idesc_mxf4(256, kBN, 2 * (i & 1)), t_word, t_word + 4,
+                             (k + kk > 0 || i > 0) ? 1u : 0u);
+            }
           }
-          if (!ok) break;
+          if (++set == S::kSets) { set = 0; set_phase ^= 1; }
           umma_commit_pair_mask(smem_u32(&empty_bar[stage]), 3);
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
         if (ok) umma_commit_pair_mask(smem_u32(&tmem_full_bar[it & 1]), 3);
+      }
+    }
+  } else if (warp >= 6) {
+    // A stage's scales: the 16-byte line of this lane in every scale tile is four columns of TMEM.  A set of columns is free
+    // once the products of the stage kSets before are done, which is what that stage's "empty" barrier says.
+    const int quad = warp & 3;
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + S::kScaleCol;
+    int stage = 0, set = 0, old_stage = 0;
+    uint32_t phase = 0, old_phase = 0;
+    long long used = 0;
+    bool ok = true;
+    for (int t = pair_id; ok && t < num_tiles; t += num_pairs) {
+      for (int k = 0; k < p.k_steps; k += kKPer) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&scales_full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL));
+        if (!ok) break;
+        const uint8_t* ss = smem + stage * S::kStageBytes + S::kABytes + S::kBBytes;
+        alignas(16) uint32_t r[S::kSetCols];
+#pragma unroll
+        for (int w = 0; w < 2 * kKPer; ++w) {
+          *reinterpret_cast<uint4*>(&r[w * S::kWordCols]) = *reinterpret_cast<const uint4*>(ss + w * kMxScaleTile + lane * 16);
+#pragma unroll
+          for (int b = 0; b < S::kBTiles; ++b)
+            *reinterpret_cast<uint4*>(&r[w * S::kWordCols + 4 + 4 * b]) =
+                *reinterpret_cast<const uint4*>(ss + S::kAScales + (b * 2 * kKPer + w) * kMxScaleTile + lane * 16);
+        }
+        if (used >= S::kSets) {
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty_bar[old_stage]), old_phase, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY));
+          if (!ok) break;
+          tc_fence_after();
+          if (++old_stage == kStages) { old_stage = 0; old_phase ^= 1; }
+        }
+        ++used;
+#pragma unroll
+        for (int c = 0; c < S::kSetCols; c += 8) tmem_st_32x32b_x8(t_lane + set * S::kSetCols + c, &r[c]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(smem_u32(&scales_set_bar[set]), 0);
+        if (++set == S::kSets) set = 0;
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
   } else {
@@ -239,21 +280,25 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::kAcc1;
       uint32_t words[kBN / 128] = {};                  // MX_MX: this row's scales
 #pragma unroll 1
-      for (int step = 0; step < kBN / 64; ++step) {
+      for (int half = 0; half < kBN / 128; ++half) {
         // accumulator 0 of 256 columns shares its last ones, accumulator 1 its first
-        const int c = S::kShared && acc == 0 ? (step == 0 ? 192 : 64 * (step - 1)) : 64 * step;
-        uint32_t r[2][32];
+        const int c_half = S::kShared && acc == 0 ? 128 - 128 * half : 128 * half;
+        uint32_t all[4][32];
         __syncwarp();
-        tmem_ld_32x32b_x32(taddr + c, r[0]);
-        tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(taddr + c_half + 32 * i, all[i]);
         tmem_ld_wait();
-        if (step == (S::kShared ? 0 : kBN / 64 - 1)) {
+        if (half == 0) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_remote(smem_u32(&tmem_free_bar[S::kShared ? 0 : acc]), 0);
         }
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+        const int c = c_half + 64 * step;
+        uint32_t (&r)[2][32] = *reinterpret_cast<uint32_t (*)[2][32]>(&all[2 * step]);
         if constexpr (kOut == MX_MX) {
-          if (step == 0) {
+          if (half == 0 && step == 0) {
             if (lane == 0) tma_store_wait_read<0>();   // the tile before has left the buffer
             __syncwarp();
           }
@@ -327,6 +372,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         } else {
           store_rows<kOut>(p, buf, r[0], row0, n0 + c, lane);
           store_rows<kOut>(p, buf, r[1], row0, n0 + c + 32, lane);
+        }
         }
       }
       if constexpr (kOut == MX_MX) {

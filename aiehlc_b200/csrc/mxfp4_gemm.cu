@@ -28,6 +28,7 @@ struct MxGemmParams {
   int vec_ok;               // four results at a time may be stored as a vector
   int m_tiles, n_tiles;
   int group_m;              // CTA pairs: row blocks walked before the next column block
+  int wide_boxes;           // CTA pairs: one box brings all steps of a stage (K a multiple of 256)
   int tile_store;           // CTA pairs: results leave as TMA tile stores
   int* status;
   int debug;                // 3: the producer withholds its loads, so every wait runs out
@@ -364,16 +365,17 @@ int encode_result_map(aiehlc_ctx* ctx, CUtensorMap* map, const MxGemmCall& c) {
   return AIEHLC_OK;
 }
 
-template <int kBN, int kKPer, int kOut>
+template <int kBN, int kOut>
 int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStream_t st) {
-  using S = MxPairShape<kBN, kKPer>;
+  using S = MxPairShape<kBN>;
   CUtensorMap ma, mb, mas, mbs, mc;
-  if constexpr (kKPer == 1) {
-    if (int rc = encode_codes_map(ctx, &ma, c.A, c.M, c.K, 128)) return rc;
-    if (int rc = encode_codes_map(ctx, &mb, c.B, c.N, c.K, kBN / 2)) return rc;
-  } else {
+  p.wide_boxes = c.K % kStepK == 0 && ctx->k_per_load != 1;
+  if (p.wide_boxes) {
     if (int rc = encode_codes_map_3d(ctx, &ma, c.A, c.M, c.K, 128, kKPer)) return rc;
     if (int rc = encode_codes_map_3d(ctx, &mb, c.B, c.N, c.K, kBN / 2, kKPer)) return rc;
+  } else {
+    if (int rc = encode_codes_map(ctx, &ma, c.A, c.M, c.K, 128)) return rc;
+    if (int rc = encode_codes_map(ctx, &mb, c.B, c.N, c.K, kBN / 2)) return rc;
   }
   if (int rc = encode_scales_map(ctx, &mas, c.As, c.M, c.K, 1, kKPer)) return rc;
   if (int rc = encode_scales_map(ctx, &mbs, c.Bs, c.N, c.K, S::kBTiles, kKPer)) return rc;
@@ -388,7 +390,7 @@ int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStrea
   p.n_tiles = (c.N + kBN - 1) / kBN;
   p.group_m = ctx->group_m > 0 ? ctx->group_m : 8;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-  auto kern = mx_gemm_pair_kernel<kBN, kKPer, kOut>;
+  auto kern = mx_gemm_pair_kernel<kBN, kOut>;
   KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
   if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::kTotal, &ks.smem_attr)) return rc;
   cudaLaunchConfig_t cfg{};
@@ -424,11 +426,10 @@ int launch_out(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
   p.status = ctx->d_status;
   p.debug = ctx->debug_mode;
   if (c.M > 128 || ctx->pair_mode == 1) {
-    const bool two = c.K % kStepK == 0 && c.K >= 2 * kStepK && ctx->k_per_load != 1;
     const long long tiles = ((c.M + 255LL) / 256) * ((c.N + 255LL) / 256);
     if (ctx->force_tile_n == 128 || (ctx->force_tile_n == 0 && tiles * 2 <= ctx->usable_sms() / 2))
-      return two ? launch_pair<128, 2, kOut>(ctx, c, p, st) : launch_pair<128, 1, kOut>(ctx, c, p, st);
-    return two ? launch_pair<256, 2, kOut>(ctx, c, p, st) : launch_pair<256, 1, kOut>(ctx, c, p, st);
+      return launch_pair<128, kOut>(ctx, c, p, st);
+    return launch_pair<256, kOut>(ctx, c, p, st);
   }
   if (c.M <= 16) return launch_narrow<16, kOut>(ctx, c, p, st);
   if (c.M <= 32) return launch_narrow<32, kOut>(ctx, c, p, st);

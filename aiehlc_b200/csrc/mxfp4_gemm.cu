@@ -186,35 +186,39 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     }
     if (!ok)
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land before the CTA retires
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int k = k_first; k < k_last; ++k) {
-      ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL));
       if (!ok) break;
       tc_fence_after();
       const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
       const uint32_t scales = at + S::kBBytes + S::kABytes;
       const uint32_t t_scales = tmem_base + kTN + stage * 16;  // 8 columns of B's scales, 8 of A's; free like the stage
       const int mmas = min(kStepK, p.K - k * kStepK + kMmaK - 1) / kMmaK;
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-        if (2 * w < mmas) {
-          tmem_copy_scales<1>(t_scales + 4 * w, make_scale_desc(scales + w * kMxScaleTile));
-          tmem_copy_scales<1>(t_scales + 8 + 4 * w, make_scale_desc(scales + kStepScales + w * kMxScaleTile));
-        }
+      const uint64_t sdesc = make_scale_desc(scales);
       const uint64_t bdesc = make_kmajor_desc(at, 1024, 2);
       const uint64_t adesc = make_kmajor_desc(at + S::kBBytes, 1024, 2);
+      if (elect_one()) {
 #pragma unroll
-      for (int i = 0; i < kStepK / kMmaK; ++i)
-        if (i < mmas)
-          umma_mxf4<1>(tmem_base, bdesc + 2 * i, adesc + 2 * i, make_idesc_mxf4(128, kTN, 2 * (i & 1)),
-                       t_scales + 4 * (i >> 1), t_scales + 8 + 4 * (i >> 1), (k > k_first || i > 0) ? 1u : 0u);
-      umma_commit(smem_u32(&empty_bar[stage]));
+        for (int w = 0; w < 2; ++w)
+          if (2 * w < mmas) {
+            tmem_copy_scales<1>(t_scales + 4 * w, sdesc + w * (kMxScaleTile >> 4));
+            tmem_copy_scales<1>(t_scales + 8 + 4 * w, sdesc + ((kStepScales + w * kMxScaleTile) >> 4));
+          }
+#pragma unroll
+        for (int i = 0; i < kStepK / kMmaK; ++i)
+          if (i < mmas)
+            umma_mxf4<1>(tmem_base, bdesc + 2 * i, adesc + 2 * i, make_idesc_mxf4(128, kTN, 2 * (i & 1)),
+                         t_scales + 4 * (i >> 1), t_scales + 8 + 4 * (i >> 1), (k > k_first || i > 0) ? 1u : 0u);
+        umma_commit(smem_u32(&empty_bar[stage]));
+      }
+      __syncwarp();
       if (++stage == S::kStages) { stage = 0; phase ^= 1; }
     }
-    if (ok) umma_commit(smem_u32(done_bar));
+    if (ok && elect_one()) umma_commit(smem_u32(done_bar));
   }
   __syncwarp();
 

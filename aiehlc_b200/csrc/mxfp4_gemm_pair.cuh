@@ -184,7 +184,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land before the CTA retires
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       int stage = 0;
       uint32_t phase = 0;
       int set = 0;
@@ -196,38 +196,37 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         // it signals is that it has read the shared ones of the last tile, for which it was through with the tile before.
         if constexpr (S::kShared) ok = it == 0 || mbar_wait(smem_u32(tmem_free_bar), (it - 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
         else ok = it < 2 || mbar_wait(smem_u32(&tmem_free_bar[it & 1]), ((it >> 1) - 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
+        ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (it & 1) * S::kAcc1;
         for (int k = 0; k < p.k_steps; k += kKPer) {
-          ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL);
-          if (!ok) break;
-          tc_fence_after();
-          ok = mbar_wait(smem_u32(&scales_set_bar[set]), set_phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+          ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL) &&
+               mbar_wait(smem_u32(&scales_set_bar[set]), set_phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+          ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * S::kStageBytes);
-          const uint32_t sb = sa + S::kABytes;
+          const uint64_t adesc = make_kmajor_desc(sa, 1024, 2);
+          const uint64_t bdesc = make_kmajor_desc(sa + S::kABytes, 1024, 2);
           const uint32_t t_scales = tmem_base + S::kScaleCol + set * S::kSetCols;
+          const int mmas = min(kKPer * kStepK, p.K - k * kStepK + kMmaK - 1) / kMmaK;
+          if (elect_one()) {
+            constexpr int kPerStep = kStepK / kMmaK;
 #pragma unroll
-          for (int kk = 0; kk < kKPer; ++kk) {
-            if (k + kk >= p.k_steps) break;
-            const int mmas = min(kStepK, p.K - (k + kk) * kStepK + kMmaK - 1) / kMmaK;
-            const uint64_t adesc = make_kmajor_desc(sa + kk * S::kABlock, 1024, 2);
-            const uint64_t bdesc = make_kmajor_desc(sb + kk * S::kBBlock, 1024, 2);
-#pragma unroll
-            for (int i = 0; i < kStepK / kMmaK; ++i) {
-              const uint32_t t_word = t_scales + (2 * kk + (i >> 1)) * S::kWordCols;
+            for (int i = 0; i < kKPer * kPerStep; ++i)
               if (i < mmas)
-                umma_mxf4<2>(d_tmem, adesc + 2 * i, bdesc + 2 * i, make_idesc_mxf4(256, kBN, 2 * (i & 1)), t_word, t_word + 4,
-                             (k + kk > 0 || i > 0) ? 1u : 0u);
-            }
+                umma_mxf4<2>(d_tmem, adesc + ((i / kPerStep) * (S::kABlock >> 4) + 2 * (i % kPerStep)),
+                             bdesc + ((i / kPerStep) * (S::kBBlock >> 4) + 2 * (i % kPerStep)), make_idesc_mxf4(256, kBN, 2 * (i & 1)),
+                             t_scales + (i >> 1) * S::kWordCols, t_scales + (i >> 1) * S::kWordCols + 4, (k > 0 || i > 0) ? 1u : 0u);
+            umma_commit_pair_mask(smem_u32(&empty_bar[stage]), 3);
           }
+          __syncwarp();
           if (++set == S::kSets) { set = 0; set_phase ^= 1; }
-          umma_commit_pair_mask(smem_u32(&empty_bar[stage]), 3);
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
-        if (ok) umma_commit_pair_mask(smem_u32(&tmem_full_bar[it & 1]), 3);
+        if (ok && elect_one()) umma_commit_pair_mask(smem_u32(&tmem_full_bar[it & 1]), 3);
+        __syncwarp();
       }
     }
   } else if (warp >= 6) {

@@ -35,6 +35,14 @@ __device__ __forceinline__ unsigned long long globaltimer_ns() {
   return t;
 }
 
+// True in one lane of a converged warp.  Code that the whole warp walks and one elected lane issues keeps its addresses and
+// descriptors in uniform registers; under `if (lane == 0)` the compiler has to move each operand there for every instruction.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // ------------------------------------------------ programmatic dependent launch
 // A kernel launched with the programmatic-stream-serialization attribute may start while the
 // kernel before it in the stream is still draining.  Everything before pdl_wait() (barrier set-up,

@@ -11,7 +11,6 @@ A[M][K] row-major, B stored [N][K], C[M][N] row-major.
 from __future__ import annotations
 
 import ctypes as C
-from typing import NamedTuple
 
 import numpy as np
 
@@ -61,19 +60,65 @@ def plan_tile_order(M: int, N: int, K: int, kind: str = "int8", num_shards: int 
     return rb[:got], cb[:got], int(slots.value)
 
 
-class MxFp4(NamedTuple):
+class MxFp4:
     """A microscaled 4-bit matrix [rows][cols]: 32 consecutive elements of a row share a power of two (the format and the
-    layout of the two arrays: aiehlc_b200.h)."""
-    codes: "object"    # uint8 [rows][16 * ceil(cols / 32)]
-    scales: "object"   # uint8 [512 * ceil(rows / 128) * ceil(cols / 128)]
-    rows: int
-    cols: int
+    layout of the two arrays: aiehlc_b200.h).
+
+    codes   uint8 [rows][16 * ceil(cols / 32)]
+    scales  uint8 [512 * ceil(rows / 128) * ceil(cols / 128)]
+
+    Both are CUDA tensors on one device.  Sizes and types are checked here, once; the calls take the matrix as it is.  One that
+    a call makes keeps both arrays in one allocation."""
+
+    __slots__ = ("rows", "cols", "device_index", "_codes", "_scales", "_whole", "_at")
+
+    def __init__(self, codes, scales, rows: int, cols: int):
+        import torch
+        if rows < 0 or cols < 0:
+            raise ValueError("MxFp4: negative size")
+        index = codes.get_device() if isinstance(codes, torch.Tensor) else -1
+        for t, n, size in ((codes, "codes", rows * ((cols + 31) // 32 * 16)),
+                           (scales, "scales", (rows + 127) // 128 * ((cols + 127) // 128) * 512)):
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.uint8 or t.get_device() != index or index < 0:
+                raise TypeError(f"MxFp4: {n}: expected a uint8 CUDA tensor, codes and scales on one device")
+            if t.numel() != size or not t.is_contiguous():
+                raise ValueError(f"MxFp4: {n}: expected {size} contiguous bytes for {rows} x {cols}")
+        self.rows, self.cols, self.device_index = rows, cols, index
+        self._codes, self._scales, self._whole = codes, scales, None
+        self._at = (codes.data_ptr(), scales.data_ptr())
+
+    @classmethod
+    def _of(cls, blank, rows: int, cols: int, index: int) -> "MxFp4":
+        """An unfilled one; `blank` is a uint8 tensor of the device."""
+        q = cls.__new__(cls)
+        size = rows * ((cols + 31) // 32 * 16)
+        whole = blank.new_empty(size + (rows + 127) // 128 * ((cols + 127) // 128) * 512)
+        at = whole.data_ptr()
+        q.rows, q.cols, q.device_index, q._codes, q._scales, q._whole, q._at = rows, cols, index, None, None, whole, (at, at + size)
+        return q
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "MxFp4":
+        """An unfilled one, for the `out` of a call."""
         import torch
-        return cls(torch.empty((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=device),
-                   torch.empty(-(-rows // 128) * -(-cols // 128) * 512, dtype=torch.uint8, device=device), rows, cols)
+        if rows < 0 or cols < 0:
+            raise ValueError("MxFp4: negative size")
+        blank = torch.empty(0, dtype=torch.uint8, device=device)
+        if not blank.is_cuda:
+            raise TypeError("MxFp4: expected a CUDA device")
+        return cls._of(blank, rows, cols, blank.get_device())
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            self._codes = self._whole[:self._at[1] - self._at[0]].view(self.rows, (self.cols + 31) // 32 * 16)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._scales = self._whole[self._at[1] - self._at[0]:]
+        return self._scales
 
 
 class Context:
@@ -354,26 +399,39 @@ class Context:
     # ------------------------------------------------ microscaled 4-bit matrices
     # These are called once per layer and token, where the work around a launch counts as much as the launch: results are
     # allocated from an empty tensor of their type (1.8 us against 2.4 us for torch.empty with a device) and not checked again,
-    # the stream is taken as a number (0.1 us against 1.5 us), and torch is looked up once.
+    # a quantised matrix is one allocation, the stream is taken as a number (0.1 us against 1.5 us), torch is looked up once.
     def _mx_setup(self):
         import torch
         self._torch = torch
         self._blank = {t: torch.empty(0, dtype=t, device=torch.device("cuda", self.device))
                        for t in (torch.uint8, torch.float32, torch.bfloat16, torch.float16)}
+        self._bytes = self._blank[torch.uint8]
         self._types = {torch.float32: _capi.TYPE_F32, torch.bfloat16: _capi.TYPE_BF16, torch.float16: _capi.TYPE_F16}
         self._raw_stream = torch._C._cuda_getCurrentRawStream
         return torch
 
-    def _new(self, rows, cols, dtype):
-        blank = self._blank.get(dtype)
-        if blank is None or dtype not in self._types:
-            raise TypeError(f"dtype: expected float32, bfloat16 or float16, got {dtype}")
-        return blank.new_empty((rows, cols))
+    def _mx(self, q, name):
+        """(codes, scales) addresses of a quantised matrix."""
+        if not isinstance(q, MxFp4):
+            raise TypeError(f"{name}: expected an MxFp4")
+        if q.device_index != self.device:
+            raise TypeError(f"{name}: expected a matrix on device {self.device}")
+        return q._at
 
-    def _new_mx(self, rows, cols):
-        blank = self._blank[self._torch.uint8]
-        return MxFp4(blank.new_empty((rows, (cols + 31) // 32 * 16)),
-                     blank.new_empty((rows + 127) // 128 * ((cols + 127) // 128) * 512), rows, cols)
+    def _result(self, out, dtype, rows, cols, name):
+        """(tensor, address, type, row pitch) of a rows x cols result: `out`, checked, or a new one."""
+        if out is None:
+            if dtype is None:
+                dtype = self._torch.bfloat16
+            kind = self._types.get(dtype)
+            if kind is None:
+                raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {dtype}")
+            out = self._blank[dtype].new_empty((rows, cols))
+            return out, out.data_ptr(), kind, cols
+        addr, kind, r, c, ld = self._rows_of(out, "out")
+        if r != rows or c != cols or (dtype is not None and out.dtype != dtype):
+            raise ValueError(f"{name}: out has another shape or type")
+        return out, addr, kind, ld
 
     def _rows_of(self, t, name):
         """(address, type, rows, cols, row pitch) of a matrix whose rows are dense; rows may be further apart."""
@@ -392,23 +450,6 @@ class Context:
             raise ValueError(f"{name}: the elements of a row must be contiguous and rows must not overlap")
         return t.data_ptr(), kind, rows, cols, ld
 
-    def _mx(self, q, name):
-        """(codes, scales) addresses of a quantised matrix, with its sizes checked."""
-        if not isinstance(q, MxFp4):
-            raise TypeError(f"{name}: expected an MxFp4")
-        codes, scales, rows, cols = q
-        torch = self._torch
-        u8 = torch.uint8
-        for t, n in ((codes, "codes"), (scales, "scales")):
-            if not isinstance(t, torch.Tensor) or t.dtype is not u8 or t.get_device() != self.device:
-                raise TypeError(f"{name}.{n}: expected a uint8 CUDA tensor on device {self.device}")
-        if codes.numel() != rows * ((cols + 31) // 32 * 16) or not codes.is_contiguous():
-            raise ValueError(f"{name}.codes: expected {rows * ((cols + 31) // 32 * 16)} contiguous bytes for {rows} x {cols}")
-        if scales.numel() != (rows + 127) // 128 * ((cols + 127) // 128) * 512 or not scales.is_contiguous():
-            raise ValueError(f"{name}.scales: expected {(rows + 127) // 128 * ((cols + 127) // 128) * 512} contiguous bytes for "
-                             f"{rows} x {cols}")
-        return codes.data_ptr(), scales.data_ptr()
-
     def quantize_mxfp4(self, x, way: str = "rows", out=None):
         """x [rows][cols] (float32, bfloat16 or float16; rows dense, any row pitch) as MxFp4: along its "rows"; along its
         "columns" (the transposed matrix [cols][rows], its blocks 32 rows of x, which is what products over the rows of x
@@ -418,22 +459,18 @@ class Context:
         if way not in ("rows", "columns", "both"):
             raise ValueError('quantize_mxfp4: way is "rows", "columns" or "both"')
         addr, kind, rows, cols, ld = self._rows_of(x, "x")
-        q = t = qc = qs = tc = ts = None
         if out is None:
-            if way != "columns":
-                q = self._new_mx(rows, cols)
-                qc, qs = q.codes.data_ptr(), q.scales.data_ptr()
-            if way != "rows":
-                t = self._new_mx(cols, rows)
-                tc, ts = t.codes.data_ptr(), t.scales.data_ptr()
+            q = None if way == "columns" else MxFp4._of(self._bytes, rows, cols, self.device)
+            t = None if way == "rows" else MxFp4._of(self._bytes, cols, rows, self.device)
         else:
             q, t = out if way == "both" else (out, None) if way == "rows" else (None, out)
-            if q is not None:
-                qc, qs = self._mx(q, "out")
-            if t is not None:
-                tc, ts = self._mx(t, "out")
-            if (q is not None and (q.rows, q.cols) != (rows, cols)) or (t is not None and (t.rows, t.cols) != (cols, rows)):
-                raise ValueError("quantize_mxfp4: out has other sizes")
+            for m, r, c in ((q, rows, cols), (t, cols, rows)):
+                if m is not None:
+                    self._mx(m, "out")
+                    if m.rows != r or m.cols != c:
+                        raise ValueError("quantize_mxfp4: out has other sizes")
+        qc, qs = q._at if q is not None else (None, None)
+        tc, ts = t._at if t is not None else (None, None)
         rc = self._lib.aiehlc_quantize_mxfp4_dev(self._h, addr, kind, rows, cols, ld, qc, qs, tc, ts, self._raw_stream(self.device))
         if rc:
             _capi.check(rc)
@@ -441,14 +478,11 @@ class Context:
 
     def dequantize_mxfp4(self, q, dtype=None, out=None):
         """The values of a quantised matrix (exact in float32 and, the default, bfloat16; float16 rounds)."""
-        torch = self._torch or self._mx_setup()
+        if self._torch is None:
+            self._mx_setup()
         codes, scales = self._mx(q, "q")
-        if out is None:
-            out = self._new(q.rows, q.cols, dtype or torch.bfloat16)
-        addr, kind, rows, cols, ld = self._rows_of(out, "out")
-        if rows != q.rows or cols != q.cols or (dtype is not None and out.dtype != dtype):
-            raise ValueError("dequantize_mxfp4: out has another shape or type")
-        rc = self._lib.aiehlc_dequantize_mxfp4_dev(self._h, codes, scales, rows, cols, addr, kind, ld, self._raw_stream(self.device))
+        out, addr, kind, ld = self._result(out, dtype, q.rows, q.cols, "dequantize_mxfp4")
+        rc = self._lib.aiehlc_dequantize_mxfp4_dev(self._h, codes, scales, q.rows, q.cols, addr, kind, ld, self._raw_stream(self.device))
         if rc:
             _capi.check(rc)
         return out
@@ -456,19 +490,16 @@ class Context:
     def gemm_mxfp4(self, A, B, dtype=None, out=None, accumulate: bool = False):
         """C = A . B^T of quantised A [M][K] and B [N][K], sums in 32-bit floating point, in dtype (default bfloat16, or
         that of `out`).  accumulate: C += A . B^T (float32 only)."""
-        torch = self._torch or self._mx_setup()
+        if self._torch is None:
+            self._mx_setup()
         if accumulate and out is None:
             raise ValueError("gemm_mxfp4: accumulate needs an existing output")
         ac, as_ = self._mx(A, "A")
         bc, bs = self._mx(B, "B")
         if A.cols != B.cols:
             raise ValueError("gemm_mxfp4: A is [M][K], B is [N][K]; K differs")
-        if out is None:
-            out = self._new(A.rows, B.rows, dtype or torch.bfloat16)
-        addr, kind, M, N, ldc = self._rows_of(out, "out")
-        if M != A.rows or N != B.rows or (dtype is not None and out.dtype != dtype):
-            raise ValueError("gemm_mxfp4: out has another shape or type")
-        rc = self._lib.aiehlc_gemm_mxfp4_dev(self._h, ac, as_, bc, bs, addr, kind, M, N, A.cols, ldc, 1 if accumulate else 0,
+        out, addr, kind, ldc = self._result(out, dtype, A.rows, B.rows, "gemm_mxfp4")
+        rc = self._lib.aiehlc_gemm_mxfp4_dev(self._h, ac, as_, bc, bs, addr, kind, A.rows, B.rows, A.cols, ldc, 1 if accumulate else 0,
                                              self._raw_stream(self.device))
         if rc:
             _capi.check(rc)
@@ -484,12 +515,12 @@ class Context:
         if A.cols != B.cols:
             raise ValueError("gemm_mxfp4_mxfp4: A is [M][K], B is [N][K]; K differs")
         if out is None:
-            out = self._new_mx(A.rows, B.rows)
-            cc, cs = out.codes.data_ptr(), out.scales.data_ptr()
+            out = MxFp4._of(self._bytes, A.rows, B.rows, self.device)
         else:
-            cc, cs = self._mx(out, "out")
+            self._mx(out, "out")
             if out.rows != A.rows or out.cols != B.rows:
                 raise ValueError("gemm_mxfp4_mxfp4: out has other sizes")
+        cc, cs = out._at
         rc = self._lib.aiehlc_gemm_mxfp4_mxfp4_dev(self._h, ac, as_, bc, bs, cc, cs, A.rows, B.rows, A.cols,
                                                    self._raw_stream(self.device))
         if rc:

@@ -391,11 +391,19 @@ def test_refusals(ctx):
     with pytest.raises(ValueError, match="shape or type"):
         ctx.gemm_mxfp4(q, q, torch.float32, out=torch.zeros(40, 40, dtype=torch.bfloat16, device=DEV))
     with pytest.raises(ValueError, match="bytes for"):
-        ctx.dequantize_mxfp4(q._replace(cols=65))
+        MxFp4(q.codes, q.scales, 40, 65)
     with pytest.raises(ValueError, match="bytes for"):
-        ctx.dequantize_mxfp4(q._replace(rows=129))
+        MxFp4(torch.empty(129, 32, dtype=torch.uint8, device=DEV), q.scales, 129, 64)
+    with pytest.raises(ValueError, match="negative"):
+        MxFp4.empty(-1, 64, DEV)
+    with pytest.raises(ValueError, match="contiguous"):
+        MxFp4(torch.empty(32, 40, dtype=torch.uint8, device=DEV).t(), q.scales, 40, 64)
     with pytest.raises(TypeError, match="uint8"):
-        ctx.dequantize_mxfp4(q._replace(scales=q.scales.float()))
+        MxFp4(q.codes, q.scales.float(), 40, 64)
+    with pytest.raises(TypeError, match="one device"):
+        MxFp4(q.codes, q.scales.cpu(), 40, 64)
+    with pytest.raises(TypeError, match="CUDA device"):
+        MxFp4.empty(4, 64, "cpu")
     with pytest.raises(Exception, match="16-byte"):
-        ctx.dequantize_mxfp4(q._replace(codes=torch.empty(40 * 32 + 8, dtype=torch.uint8, device=DEV)[8:].view(40, 32)))
+        ctx.dequantize_mxfp4(MxFp4(torch.empty(40 * 32 + 8, dtype=torch.uint8, device=DEV)[8:].view(40, 32), q.scales, 40, 64))
     assert ctx.launch_count == before and ctx.sync() == 0

@@ -38,20 +38,14 @@ __device__ __forceinline__ int mx_scale_of(uint32_t max_bits) {
   const int e = static_cast<int>(max_bits >> 23);
   return e == 255 ? kMxNan : (e > 2 ? e - 2 : 0);
 }
-// 2^-e for scale byte s: exact, and normal for every scale mx_scale_of gives (s <= 252).  0 for a NaN block, whose
-// codes are written as zeros.
-__device__ __forceinline__ float mx_inverse(int s) {
-  return s == kMxNan ? 0.0f : __uint_as_float(static_cast<uint32_t>(254 - s) << 23);
-}
+// 2^-e for scale byte s: exact, and normal for every finite scale mx_scale_of gives (s <= 252).
+__device__ __forceinline__ float mx_inverse(int s) { return __uint_as_float(static_cast<uint32_t>(254 - s) << 23); }
 // 2^e for scale byte s (2^-127 is subnormal); NaN for 255.
 __device__ __forceinline__ float mx_scale_value(int s) {
   return __uint_as_float(s == kMxNan ? 0x7FC00000u : s == 0 ? 0x00400000u : static_cast<uint32_t>(s) << 23);
 }
-// 0 * inf and 0 * NaN are NaN: elements of a NaN block are replaced before they are converted.
-__device__ __forceinline__ float mx_scaled(float x, float inv) { return inv == 0.0f ? 0.0f : x * inv; }
-
-// Eight values (already divided by the scale) to eight codes, v[0] in the low four bits.  The conversion rounds
-// to nearest, ties to even, and saturates at 6.
+// Eight values, already divided by the scale, to eight codes, v[0] in the low four bits.  The conversion rounds to
+// nearest, ties to even, and saturates at 6.  (A block that is NaN has its codes replaced by zeros.)
 __device__ __forceinline__ uint32_t mx_codes8(const float (&v)[8]) {
   uint32_t r;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
@@ -80,11 +74,7 @@ __device__ __forceinline__ void mx_decode8(uint32_t codes, __half2 (&h)[4]) {
   h[3] = *reinterpret_cast<__half2*>(&r3);
 }
 
-// One element of each type the entry points take (AIEHLC_TYPE_*).
-template <typename T> __device__ __forceinline__ float mx_to_float(T v);
-template <> __device__ __forceinline__ float mx_to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float mx_to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float mx_to_float<__half>(__half v) { return __half2float(v); }
+// One element of each type the entry points take (AIEHLC_TYPE_*), rounded to nearest even.
 template <typename T> __device__ __forceinline__ T mx_from_float(float v);
 template <> __device__ __forceinline__ float mx_from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 mx_from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }

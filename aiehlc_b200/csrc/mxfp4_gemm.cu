@@ -106,8 +106,8 @@ __device__ __forceinline__ void store_blocks(const MxGemmParams& p, int m, int n
   const int s = mx_scale_of(most);
   const float inv = mx_inverse(s);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = mx_scaled(f[i], inv);
-  const uint16_t codes = static_cast<uint16_t>(mx_codes8(f));
+  for (int i = 0; i < 4; ++i) f[i] *= inv;
+  const uint16_t codes = s == kMxNan ? 0 : static_cast<uint16_t>(mx_codes8(f));
   const int blocks = static_cast<int>(mx_blocks(p.N));
   const bool there = n / kMxBlock < blocks;
   if (there) *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.C) + static_cast<long long>(m) * blocks * 16 + n / 2) = codes;

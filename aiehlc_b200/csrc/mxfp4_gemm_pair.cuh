@@ -325,8 +325,8 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             for (int g = 0; g < 4; ++g) {
               float f[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] = mx_scaled(__uint_as_float(r[h][8 * g + j]), inv);
-              w[g] = mx_codes8(f);
+              for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(r[h][8 * g + j]) * inv;
+              w[g] = s == kMxNan ? 0 : mx_codes8(f);
             }
             const int piece = c / 32 + h;              // 16 bytes of codes per block
             *reinterpret_cast<uint4*>(buf + lane * (kBN / 2) + ((piece ^ (kBN == 256 ? swz : (lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);

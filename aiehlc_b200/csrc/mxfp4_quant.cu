@@ -13,20 +13,62 @@ constexpr int kLanesPerRow = kTile / 8;                      // a thread holds 8
 constexpr int kRowsPerPass = kQuantThreads / kLanesPerRow;   // 16
 constexpr int kPasses = kTile / kRowsPerPass;                // 8
 
-// Eight consecutive elements of a row; elements at or past `cols` are zero.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T* row, long long col, long long cols, T (&v)[8]) {
-  if (kVec && col + 8 <= cols) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<uint4*>(&v[0]) = *reinterpret_cast<const uint4*>(row + col);
-      *reinterpret_cast<uint4*>(&v[4]) = *reinterpret_cast<const uint4*>(row + col + 4);
-    } else {
-      *reinterpret_cast<uint4*>(&v[0]) = *reinterpret_cast<const uint4*>(row + col);
-    }
-  } else {
+// Eight consecutive elements as they come from memory, two to a register for the 16-bit types.
+template <typename T>
+struct Eight {
+  static constexpr int kWords = 2 * static_cast<int>(sizeof(T));
+  uint32_t w[kWords];
+};
+template <typename T> __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b);   // of two pairs, as magnitudes
+template <> __device__ __forceinline__ uint32_t max_abs2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  a &= 0x7FFF7FFFu;
+  b &= 0x7FFF7FFFu;
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <> __device__ __forceinline__ uint32_t max_abs2<__half>(uint32_t a, uint32_t b) {
+  a &= 0x7FFF7FFFu;
+  b &= 0x7FFF7FFFu;
+  const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <typename T> __device__ __forceinline__ float2 split2(uint32_t w);
+template <> __device__ __forceinline__ float2 split2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <> __device__ __forceinline__ float2 split2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// Largest magnitude as float bits; a NaN or infinity keeps the exponent 255.
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(const Eight<T>& v) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? row[col + i] : mx_from_float<T>(0.0f);
+    for (int i = 0; i < 8; ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+    const uint32_t m = max_abs2<T>(max_abs2<T>(v.w[0], v.w[1]), max_abs2<T>(v.w[2], v.w[3]));
+    const float2 f = split2<T>(m);
+    return max(__float_as_uint(f.x), __float_as_uint(f.y)) & 0x7FFFFFFFu;
   }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const Eight<T>& v, int s) {
+  const float inv = mx_inverse(s);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(v.w[i]) * inv;
+      f[i + 1] = __uint_as_float(v.w[i + 1]) * inv;
+    } else {
+      const float2 p = split2<T>(v.w[i >> 1]);
+      f[i] = p.x * inv;
+      f[i + 1] = p.y * inv;
+    }
+  }
+  return s == kMxNan ? 0u : mx_codes8(f);
 }
 
 // One pass over the matrix.  Bound by memory: sizeof(T) bytes read and 17/32 written per element and direction.
@@ -34,16 +76,18 @@ __device__ __forceinline__ void load8(const T* row, long long col, long long col
 //   columns: the tile turns through shared memory; a thread takes 32 rows of two neighbouring columns, and the codes
 //            of a column's four blocks leave as 64 contiguous bytes
 // A 128 x 128 tile makes exactly one 512-byte scale tile each way, which leaves as one contiguous store.
+// Where rows do not start on 16 bytes (kVec false) the tile comes in element by element, neighbouring lanes on neighbouring
+// elements, and the rows are read back from shared memory.
 template <typename T, bool kVec, bool kRows, bool kCols>
-__global__ void __launch_bounds__(kQuantThreads)
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 3)
 mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long long ld, uint8_t* __restrict__ q,
                    uint8_t* __restrict__ qs, uint8_t* __restrict__ t, uint8_t* __restrict__ ts, int col_tiles) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* row_scales = smem;                        // 512 bytes
   uint8_t* col_scales = smem + kMxScaleTile;         // 512 bytes
-  uint8_t* turned = smem + 2 * kMxScaleTile;         // codes along the columns, [128][64 + 16]: the pad spreads the banks
-  constexpr int kTurnedPitch = 80;
-  T* tile = reinterpret_cast<T*>(smem + 2 * kMxScaleTile + kTile * kTurnedPitch);  // [128][128]
+  T* tile = reinterpret_cast<T*>(smem + 2 * kMxScaleTile);                          // [128][128]
+  uint8_t* turned = smem + 2 * kMxScaleTile + kTile * kTile * sizeof(T);            // codes along the columns
+  constexpr int kPieces = static_cast<int>(sizeof(T)) / 2;   // 16-byte pieces of eight elements
 
   pdl_launch_dependents();
   pdl_wait();
@@ -56,48 +100,73 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
   const int line = tid / kLanesPerRow;
   const long long col = c0 + sub * 8;
   const long long blocks = mx_blocks(cols);
+  const int rows_here = static_cast<int>(min(static_cast<long long>(kTile), rows - r0));
 
-  alignas(16) T v[kPasses][8];
-#pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const long long r = r0 + p * kRowsPerPass + line;
-    if (r < rows) load8<T, kVec>(x + r * ld, col, cols, v[p]);
-    else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[p][i] = mx_from_float<T>(0.0f);
-    }
-  }
-  if constexpr (kCols) {
+  Eight<T> v[kPasses];
+  if constexpr (kVec) {
+    const bool whole = col + 8 <= cols;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      T* dst = tile + (p * kRowsPerPass + line) * kTile + sub * 8;
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(&v[p][0]);
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 4) = *reinterpret_cast<const uint4*>(&v[p][4]);
+      const int r = p * kRowsPerPass + line;
+#pragma unroll
+      for (int i = 0; i < Eight<T>::kWords; ++i) v[p].w[i] = 0;
+      if (r < rows_here) {
+        const T* src = x + (r0 + r) * ld + col;
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i)
+            *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < cols) {
+              if constexpr (sizeof(T) == 4) v[p].w[i] = reinterpret_cast<const uint32_t*>(src)[i];
+              else v[p].w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(src)[i]) << (16 * (i & 1));
+            }
+        }
+      }
+    }
+    if constexpr (kCols) {
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+          reinterpret_cast<uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * 8)[i] = *reinterpret_cast<const uint4*>(&v[p].w[4 * i]);
+    }
+  } else {
+    const int c = tid & (kTile - 1);
+    const bool col_there = c0 + c < cols;
+#pragma unroll 1
+    for (int r = tid / kTile; r < kTile; r += 32) {
+      T e[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        e[i] = col_there && r + 2 * i < rows_here ? x[(r0 + r + 2 * i) * ld + c0 + c] : mx_from_float<T>(0.0f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) tile[(r + 2 * i) * kTile + c] = e[i];
+    }
+    if constexpr (kRows) {
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+          *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = reinterpret_cast<const uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * 8)[i];
     }
   }
   if constexpr (kRows) {
+    const long long block = c0 / kMxBlock + sub / 4;
+    uint8_t* dst = q + r0 * blocks * 16 + col / 2;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      const int in_tile = p * kRowsPerPass + line;
-      float f[8];
-      uint32_t most = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        f[i] = mx_to_float(v[p][i]);
-        most = max(most, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-      }
+      const int r = p * kRowsPerPass + line;
+      uint32_t most = max_bits(v[p]);
       most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
       most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
       const int s = mx_scale_of(most);
-      const float inv = mx_inverse(s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = mx_scaled(f[i], inv);
-      const uint32_t codes = mx_codes8(f);
-      const long long r = r0 + in_tile;
-      const long long block = c0 / kMxBlock + sub / 4;
-      const bool there = r < rows && block < blocks;
-      if (there) *reinterpret_cast<uint32_t*>(q + r * blocks * 16 + col / 2) = codes;
-      if ((sub & 3) == 0) row_scales[mx_scale_word(in_tile) + sub / 4] = there ? static_cast<uint8_t>(s) : 0;
+      const bool there = r < rows_here && block < blocks;
+      if (there) *reinterpret_cast<uint32_t*>(dst + r * blocks * 16) = codes_of(v[p], s);
+      if ((sub & 3) == 0) row_scales[mx_scale_word(r) + sub / 4] = there ? static_cast<uint8_t>(s) : 0;
     }
   }
   __syncthreads();
@@ -107,17 +176,35 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
           reinterpret_cast<const uint4*>(row_scales)[tid];
   }
   if constexpr (kCols) {
+    constexpr int kTurnedPitch = 80;                 // 64 bytes of codes per column; the pad spreads the banks
     const long long row_blocks = mx_blocks(rows);
     const int pair = tid & 63, rb = tid >> 6;        // columns 2 pair, 2 pair + 1; rows 32 rb ...
     const T* src = tile + rb * kMxBlock * kTile + 2 * pair;
+    uint32_t m0, m1;
     float f0[kMxBlock], f1[kMxBlock];
-    uint32_t m0 = 0, m1 = 0;
+    if constexpr (sizeof(T) == 4) {
+      m0 = m1 = 0;
 #pragma unroll
-    for (int i = 0; i < kMxBlock; ++i) {
-      f0[i] = mx_to_float(src[i * kTile]);
-      f1[i] = mx_to_float(src[i * kTile + 1]);
-      m0 = max(m0, __float_as_uint(f0[i]) & 0x7FFFFFFFu);
-      m1 = max(m1, __float_as_uint(f1[i]) & 0x7FFFFFFFu);
+      for (int i = 0; i < kMxBlock; ++i) {
+        const float2 f = *reinterpret_cast<const float2*>(src + i * kTile);
+        f0[i] = f.x;
+        f1[i] = f.y;
+        m0 = max(m0, __float_as_uint(f.x) & 0x7FFFFFFFu);
+        m1 = max(m1, __float_as_uint(f.y) & 0x7FFFFFFFu);
+      }
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kMxBlock; ++i) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(src + i * kTile);
+        const float2 f = split2<T>(w);
+        f0[i] = f.x;
+        f1[i] = f.y;
+        m = max_abs2<T>(m, w);
+      }
+      const float2 f = split2<T>(m);
+      m0 = __float_as_uint(f.x) & 0x7FFFFFFFu;
+      m1 = __float_as_uint(f.y) & 0x7FFFFFFFu;
     }
     const bool block_there = r0 / kMxBlock + rb < row_blocks;
 #pragma unroll
@@ -130,8 +217,8 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
       for (int j = 0; j < 4; ++j) {
         float g[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = mx_scaled(h ? f1[8 * j + i] : f0[8 * j + i], inv);
-        w[j] = mx_codes8(g);
+        for (int i = 0; i < 8; ++i) g[i] = (h ? f1[8 * j + i] : f0[8 * j + i]) * inv;
+        w[j] = s == kMxNan ? 0u : mx_codes8(g);
       }
       *reinterpret_cast<uint4*>(turned + c * kTurnedPitch + rb * 16) = make_uint4(w[0], w[1], w[2], w[3]);
       col_scales[mx_scale_word(c) + rb] = block_there && c0 + c < cols ? static_cast<uint8_t>(s) : 0;
@@ -153,31 +240,42 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
 }
 
 // Values of a quantised matrix.  Bound by memory: 17/32 byte read, sizeof(T) written per element.  A CTA takes the
-// 128 x 128 elements of one scale tile; a thread turns four bytes of codes into eight values.
+// 128 x 128 elements of one scale tile; a thread turns four bytes of codes into eight values.  Where rows of y do not start
+// on 16 bytes (kVec false) a warp's two rows turn through shared memory, so that neighbouring lanes store neighbours.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ qs, long long rows, long long cols,
                      T* __restrict__ y, long long ld, int col_tiles) {
+  __shared__ __align__(16) T turned[kVec ? 1 : kQuantThreads / 32][kVec ? 1 : 2][kVec ? 8 : kTile];
   pdl_launch_dependents();
   pdl_wait();
   const long long row_tile = blockIdx.x / col_tiles;
   const int col_tile = static_cast<int>(blockIdx.x - row_tile * col_tiles);
   const long long r0 = row_tile * kTile;
+  const long long c0 = static_cast<long long>(col_tile) * kTile;
   const int sub = threadIdx.x & (kLanesPerRow - 1);
   const int line = threadIdx.x / kLanesPerRow;
-  const long long col = static_cast<long long>(col_tile) * kTile + sub * 8;
-  if (col >= cols) return;
+  const int rows_here = static_cast<int>(min(static_cast<long long>(kTile), rows - r0));
+  const int cols_here = static_cast<int>(min(static_cast<long long>(kTile), cols - c0));
+  const bool col_there = sub * 8 < cols_here;
   const long long pitch = mx_pitch(cols);
+  const uint8_t* src = q + r0 * pitch + c0 / 2 + sub * 4;
   const uint8_t* scales = qs + (row_tile * mx_words(cols) + col_tile) * kMxScaleTile + sub / 4;
+  uint32_t codes[kPasses];
+  int s[kPasses];
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int in_tile = p * kRowsPerPass + line;
-    const long long r = r0 + in_tile;
-    if (r >= rows) break;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(q + r * pitch + col / 2);
-    const float scale = mx_scale_value(scales[mx_scale_word(in_tile)]);
+    const int r = p * kRowsPerPass + line;
+    const bool there = r < rows_here && col_there;
+    codes[p] = there ? *reinterpret_cast<const uint32_t*>(src + r * pitch) : 0u;
+    s[p] = there ? scales[mx_scale_word(r)] : 0;
+  }
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int r = p * kRowsPerPass + line;
+    const float scale = mx_scale_value(s[p]);
     __half2 h[4];
-    mx_decode8(codes, h);
+    mx_decode8(codes[p], h);
     alignas(16) T v[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -185,14 +283,34 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
       v[2 * i] = mx_from_float<T>(f.x * scale);
       v[2 * i + 1] = mx_from_float<T>(f.y * scale);
     }
-    T* dst = y + r * ld + col;
-    if (kVec && col + 8 <= cols) {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(&v[0]);
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 4) = *reinterpret_cast<const uint4*>(&v[4]);
-    } else {
+    if constexpr (kVec) {
+      T* dst = y + (r0 + r) * ld + c0 + sub * 8;
+      if (r < rows_here && col_there) {
+        if (sub * 8 + 8 <= cols_here) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < cols) dst[i] = v[i];
+          for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+            reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (sub * 8 + i < cols_here) dst[i] = v[i];
+        }
+      }
+    } else {
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+        reinterpret_cast<uint4*>(&turned[warp][lane >> 4][sub * 8])[i] = reinterpret_cast<const uint4*>(v)[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = p * kRowsPerPass + 2 * warp + i;
+        T* dst = y + (r0 + row) * ld + c0;
+#pragma unroll
+        for (int j = 0; j < kTile / 32; ++j)
+          if (row < rows_here && 32 * j + lane < cols_here) dst[32 * j + lane] = turned[warp][i][32 * j + lane];
+      }
+      __syncwarp();
     }
   }
 }
@@ -213,7 +331,7 @@ cudaLaunchConfig_t tile_grid(const aiehlc_ctx* ctx, unsigned tiles, int smem, cu
 template <typename T, bool kVec, bool kRows, bool kCols>
 int quantize_as(aiehlc_ctx* ctx, const MxQuantizeCall& c, cudaStream_t st) {
   auto kern = mx_quantize_kernel<T, kVec, kRows, kCols>;
-  const int smem = 2 * kMxScaleTile + (kCols ? kTile * 80 + kTile * kTile * static_cast<int>(sizeof(T)) : 0);
+  const int smem = 2 * kMxScaleTile + (kCols || !kVec ? kTile * kTile * static_cast<int>(sizeof(T)) : 0) + (kCols ? kTile * 80 : 0);
   KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
   if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), smem, &ks.smem_attr)) return rc;
   const int col_tiles = static_cast<int>((c.cols + kTile - 1) / kTile);

@@ -9,27 +9,22 @@ namespace {
 
 constexpr int kTile = 128;          // a CTA takes 128 x 128 elements: one scale tile along the rows and one along the columns
 constexpr int kQuantThreads = 256;
-constexpr int kLanesPerRow = kTile / 8;                      // a thread holds 8 consecutive elements of a row
-constexpr int kRowsPerPass = kQuantThreads / kLanesPerRow;   // 16
-constexpr int kPasses = kTile / kRowsPerPass;                // 8
 
-// Eight consecutive elements as they come from memory, two to a register for the 16-bit types.
-template <typename T>
-struct Eight {
-  static constexpr int kWords = 2 * static_cast<int>(sizeof(T));
+// Consecutive elements of a row as they come from memory, two to a register for the 16-bit types.
+template <typename T, int kCount>
+struct alignas(16) Run {
+  static constexpr int kWords = kCount * static_cast<int>(sizeof(T)) / 4;
+  static constexpr int kPieces = kWords / 4;   // of 16 bytes
   uint32_t w[kWords];
 };
-template <typename T> __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b);   // of two pairs, as magnitudes
+// The larger magnitudes of two pairs; NaN stays NaN.
+template <typename T> __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b);
 template <> __device__ __forceinline__ uint32_t max_abs2<__nv_bfloat16>(uint32_t a, uint32_t b) {
-  a &= 0x7FFF7FFFu;
-  b &= 0x7FFF7FFFu;
-  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<__nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
   return *reinterpret_cast<const uint32_t*>(&m);
 }
 template <> __device__ __forceinline__ uint32_t max_abs2<__half>(uint32_t a, uint32_t b) {
-  a &= 0x7FFF7FFFu;
-  b &= 0x7FFF7FFFu;
-  const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  const __half2 m = __hmax2_nan(__habs2(*reinterpret_cast<__half2*>(&a)), __habs2(*reinterpret_cast<__half2*>(&b)));
   return *reinterpret_cast<const uint32_t*>(&m);
 }
 template <typename T> __device__ __forceinline__ float2 split2(uint32_t w);
@@ -40,39 +35,46 @@ template <> __device__ __forceinline__ float2 split2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 // Largest magnitude as float bits; a NaN or infinity keeps the exponent 255.
-template <typename T>
-__device__ __forceinline__ uint32_t max_bits(const Eight<T>& v) {
+template <typename T, int kCount>
+__device__ __forceinline__ uint32_t max_bits(const Run<T, kCount>& v) {
   if constexpr (sizeof(T) == 4) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
+    for (int i = 0; i < kCount; ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
     return m;
   } else {
-    const uint32_t m = max_abs2<T>(max_abs2<T>(v.w[0], v.w[1]), max_abs2<T>(v.w[2], v.w[3]));
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kCount / 2; ++i) m = max_abs2<T>(m, v.w[i]);
     const float2 f = split2<T>(m);
     return max(__float_as_uint(f.x), __float_as_uint(f.y)) & 0x7FFFFFFFu;
   }
 }
-template <typename T>
-__device__ __forceinline__ uint32_t codes_of(const Eight<T>& v, int s) {
+template <typename T, int kCount>
+__device__ __forceinline__ void codes_of(const Run<T, kCount>& v, int s, uint32_t (&codes)[kCount / 8]) {
   const float inv = mx_inverse(s);
-  float f[8];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    if constexpr (sizeof(T) == 4) {
-      f[i] = __uint_as_float(v.w[i]) * inv;
-      f[i + 1] = __uint_as_float(v.w[i + 1]) * inv;
-    } else {
-      const float2 p = split2<T>(v.w[i >> 1]);
-      f[i] = p.x * inv;
-      f[i + 1] = p.y * inv;
+  for (int g = 0; g < kCount / 8; ++g) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(v.w[8 * g + i]) * inv;
+        f[i + 1] = __uint_as_float(v.w[8 * g + i + 1]) * inv;
+      } else {
+        const float2 p = split2<T>(v.w[4 * g + (i >> 1)]);
+        f[i] = p.x * inv;
+        f[i + 1] = p.y * inv;
+      }
     }
+    codes[g] = s == kMxNan ? 0u : mx_codes8(f);
   }
-  return s == kMxNan ? 0u : mx_codes8(f);
 }
 
-// One pass over the matrix.  Bound by memory: sizeof(T) bytes read and 17/32 written per element and direction.
-//   rows   : the four lanes that hold a block agree on its maximum with two shuffles; each writes four bytes of codes
+// One pass over the matrix: sizeof(T) bytes read and 17/32 written per element and direction.  What bounds it next to memory is
+// the ALU pipe (maxima, splitting pairs, conversions; 70 % of its rate at 13 instructions an element, before a block's own
+// work was shared by two threads instead of four).
+//   rows   : the lanes that hold a block agree on its maximum with shuffles; each writes the codes of its elements
 //   columns: the tile turns through shared memory; a thread takes 32 rows of two neighbouring columns, and the codes
 //            of a column's four blocks leave as 64 contiguous bytes
 // A 128 x 128 tile makes exactly one 512-byte scale tile each way, which leaves as one contiguous store.
@@ -87,7 +89,14 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
   uint8_t* col_scales = smem + kMxScaleTile;         // 512 bytes
   T* tile = reinterpret_cast<T*>(smem + 2 * kMxScaleTile);                          // [128][128]
   uint8_t* turned = smem + 2 * kMxScaleTile + kTile * kTile * sizeof(T);            // codes along the columns
-  constexpr int kPieces = static_cast<int>(sizeof(T)) / 2;   // 16-byte pieces of eight elements
+  // Elements of a row a thread takes.  Half a block where rows are quantised (4096 x 4096 bf16, rows: 6.2 us against 8.9 us with
+  // a quarter); a quarter where the tile only passes through shared memory, where 32-byte strides cost bank
+  // conflicts (columns: 8.7 against 9.6 us; f32 both ways, 8192 x 8192: 79 against 89 us).
+  constexpr int kRun = kCols && (!kRows || sizeof(T) == 4) ? 8 : 16;
+  constexpr int kLanesPerRow = kTile / kRun;
+  constexpr int kRowsPerPass = kQuantThreads / kLanesPerRow;
+  constexpr int kPasses = kTile / kRowsPerPass;
+  using R = Run<T, kRun>;
 
   pdl_launch_dependents();
   pdl_wait();
@@ -96,42 +105,40 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
   const long long r0 = row_tile * kTile;
   const long long c0 = static_cast<long long>(col_tile) * kTile;
   const int tid = threadIdx.x;
-  const int sub = tid & (kLanesPerRow - 1);          // which eight columns of the tile
+  const int sub = tid & (kLanesPerRow - 1);
   const int line = tid / kLanesPerRow;
-  const long long col = c0 + sub * 8;
+  const long long col = c0 + sub * kRun;
   const long long blocks = mx_blocks(cols);
   const int rows_here = static_cast<int>(min(static_cast<long long>(kTile), rows - r0));
 
-  Eight<T> v[kPasses];
+  R v[kPasses];
   if constexpr (kVec) {
-    const bool whole = col + 8 <= cols;
+    const bool whole = col + kRun <= cols;
+    const T* src = x + (r0 + line) * ld + col;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int r = p * kRowsPerPass + line;
+    for (int p = 0; p < kPasses; ++p, src += kRowsPerPass * ld) {
+      const bool row_there = p * kRowsPerPass + line < rows_here;
 #pragma unroll
-      for (int i = 0; i < Eight<T>::kWords; ++i) v[p].w[i] = 0;
-      if (r < rows_here) {
-        const T* src = x + (r0 + r) * ld + col;
-        if (whole) {
+      for (int i = 0; i < R::kWords; ++i) v[p].w[i] = 0;
+      if (row_there && whole) {
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i)
-            *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = __ldg(reinterpret_cast<const uint4*>(src) + i);
-        } else {
+        for (int i = 0; i < R::kPieces; ++i)
+          *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = __ldg(reinterpret_cast<const uint4*>(src) + i);
+      } else if (row_there) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + i < cols) {
-              if constexpr (sizeof(T) == 4) v[p].w[i] = reinterpret_cast<const uint32_t*>(src)[i];
-              else v[p].w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(src)[i]) << (16 * (i & 1));
-            }
-        }
+        for (int i = 0; i < kRun; ++i)
+          if (col + i < cols) {
+            if constexpr (sizeof(T) == 4) v[p].w[i] = reinterpret_cast<const uint32_t*>(src)[i];
+            else v[p].w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(src)[i]) << (16 * (i & 1));
+          }
       }
     }
     if constexpr (kCols) {
 #pragma unroll
       for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-          reinterpret_cast<uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * 8)[i] = *reinterpret_cast<const uint4*>(&v[p].w[4 * i]);
+        for (int i = 0; i < R::kPieces; ++i)
+          reinterpret_cast<uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * kRun)[i] = *reinterpret_cast<const uint4*>(&v[p].w[4 * i]);
     }
   } else {
     const int c = tid & (kTile - 1);
@@ -150,23 +157,29 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
 #pragma unroll
       for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-          *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = reinterpret_cast<const uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * 8)[i];
+        for (int i = 0; i < R::kPieces; ++i)
+          *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = reinterpret_cast<const uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * kRun)[i];
     }
   }
   if constexpr (kRows) {
-    const long long block = c0 / kMxBlock + sub / 4;
-    uint8_t* dst = q + r0 * blocks * 16 + col / 2;
+    constexpr int kSharers = kMxBlock / kRun;        // lanes that hold a block
+    const bool block_there = c0 / kMxBlock + sub / kSharers < blocks;
+    uint8_t* dst = q + (r0 + line) * blocks * 16 + col / 2;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
+    for (int p = 0; p < kPasses; ++p, dst += kRowsPerPass * blocks * 16) {
       const int r = p * kRowsPerPass + line;
       uint32_t most = max_bits(v[p]);
-      most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-      most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+#pragma unroll
+      for (int o = 1; o < kSharers; o <<= 1) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
       const int s = mx_scale_of(most);
-      const bool there = r < rows_here && block < blocks;
-      if (there) *reinterpret_cast<uint32_t*>(dst + r * blocks * 16) = codes_of(v[p], s);
-      if ((sub & 3) == 0) row_scales[mx_scale_word(r) + sub / 4] = there ? static_cast<uint8_t>(s) : 0;
+      uint32_t codes[kRun / 8];
+      codes_of(v[p], s, codes);
+      const bool there = r < rows_here && block_there;
+      if (there) {
+        if constexpr (kRun == 16) *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
+        else *reinterpret_cast<uint32_t*>(dst) = codes[0];
+      }
+      if (sub % kSharers == 0) row_scales[mx_scale_word(r) + sub / kSharers] = there ? static_cast<uint8_t>(s) : 0;
     }
   }
   __syncthreads();
@@ -246,6 +259,9 @@ template <typename T, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ qs, long long rows, long long cols,
                      T* __restrict__ y, long long ld, int col_tiles) {
+  constexpr int kLanesPerRow = kTile / 8;
+  constexpr int kRowsPerPass = kQuantThreads / kLanesPerRow;
+  constexpr int kPasses = kTile / kRowsPerPass;
   __shared__ __align__(16) T turned[kVec ? 1 : kQuantThreads / 32][kVec ? 1 : 2][kVec ? 8 : kTile];
   pdl_launch_dependents();
   pdl_wait();

@@ -15,6 +15,8 @@ enum : int { MX_F32 = 0, MX_F32_ADD = 1, MX_BF16 = 2, MX_F16 = 3, MX_MX = 4 };
 constexpr int kStepK = 256;                    // elements of K per stage: one 128-byte swizzle span of codes
 constexpr int kStepScales = 2 * kMxScaleTile;  // two scale tiles of 4 blocks each
 constexpr int kMmaK = 64;                      // elements of K per tcgen05.mma
+constexpr int kKPer = 2;                       // steps per pipeline stage
+constexpr int kMaxSplit = 8;                   // CTAs that share the K of a narrow product
 
 struct MxGemmParams {
   int M, N, K;
@@ -28,7 +30,7 @@ struct MxGemmParams {
   int vec_ok;               // four results at a time may be stored as a vector
   int m_tiles, n_tiles;
   int group_m;              // CTA pairs: row blocks walked before the next column block
-  int wide_boxes;           // CTA pairs: one box brings all steps of a stage (K a multiple of 256)
+  int wide_boxes;           // one box brings all steps of a stage (K a multiple of 256)
   int tile_store;           // CTA pairs: results leave as TMA tile stores
   int* status;
   int debug;                // 3: the producer withholds its loads, so every wait runs out
@@ -39,17 +41,23 @@ struct MxGemmParams {
 // streams B through as many SMs as there are: each output tile (128 columns of C x kTN rows) is one cluster of
 // `split` CTAs, each of which takes an equal range of K.  The partial sums meet in distributed shared memory, added in the order
 // of the CTAs' ranks (the result does not depend on timing), and every CTA writes its share of the tile's rows.
+// A stage holds 512 elements of K: the issuing warp's wait and commit take about 400 cycles a stage, whatever it holds (a
+// product with 16 columns takes 32), and with 256 elements they set the pace.
 template <int kTN>
 struct NarrowShape {
-  static constexpr int kStages = 4;
-  static constexpr int kBBytes = 128 * 128;
-  static constexpr int kABytes = kTN * 128;
-  static constexpr int kStageBytes = kBBytes + kABytes + 2 * kStepScales;
+  static constexpr int kStages = kTN == 128 ? 2 : 3;
+  static constexpr int kBBlock = 128 * 128;                   // 256 elements of K of the tile's rows of B
+  static constexpr int kABlock = kTN * 128;
+  static constexpr int kBBytes = kBBlock * kKPer;
+  static constexpr int kABytes = kABlock * kKPer;
+  static constexpr int kScaleBytes = kStepScales * kKPer;     // of each operand
+  static constexpr int kStageBytes = kBBytes + kABytes + 2 * kScaleBytes;
   static constexpr int kPartialBytes = kTN * 128 * 4;         // over the stages, once they are done
   static constexpr int kPool = kStages * kStageBytes > kPartialBytes ? kStages * kStageBytes : kPartialBytes;
   static constexpr int kTotal = 1024 + kPool + 256;
-  static constexpr int kScaleCols = 16 * kStages;             // per stage 8 columns of each operand's scales
-  static constexpr int kTmemCols = kTN <= 64 ? 128 : 256;
+  static constexpr int kSetCols = 8 * kKPer;                  // columns of each operand's scales per stage
+  static constexpr int kScaleCols = 2 * kSetCols * kStages;
+  static constexpr int kTmemCols = kTN <= 32 ? 128 : 256;
   static_assert(kTN + kScaleCols <= kTmemCols, "TMEM");
 };
 
@@ -138,8 +146,9 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   const int tile = blockIdx.x / split;
   const int m0 = tile % p.m_tiles * kTN;
   const int n0 = tile / p.m_tiles * 128;
-  const int k_first = static_cast<int>(static_cast<long long>(p.k_steps) * rank / split);
-  const int k_last = static_cast<int>(static_cast<long long>(p.k_steps) * (rank + 1) / split);
+  const int k_stages = (p.k_steps + kKPer - 1) / kKPer;
+  const int k_first = static_cast<int>(static_cast<long long>(k_stages) * rank / split) * kKPer;
+  const int k_last = static_cast<int>(static_cast<long long>(k_stages) * (rank + 1) / split) * kKPer;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
@@ -169,18 +178,27 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     bool ok = true;
     const uint8_t* sa = p.a_scales + static_cast<long long>(m0 / 128) * p.words * kMxScaleTile;
     const uint8_t* sb = p.b_scales + static_cast<long long>(n0 / 128) * p.words * kMxScaleTile;
-    for (int k = k_first; k < k_last; ++k) {
+    for (int k = k_first; k < k_last; k += kKPer) {
       ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status, ST_TIMEOUT_EMPTY);
       if (!ok) break;
       if (p.debug != 3) {
         const uint32_t bar = smem_u32(&full_bar[stage]);
         const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
-        const uint32_t scale_bytes = (p.words - 2 * k < 2 ? 1 : 2) * kMxScaleTile;  // K may end inside the step
+        const uint32_t scales = at + S::kBBytes + S::kABytes;
+        const uint32_t scale_bytes = min(2 * kKPer, p.words - 2 * k) * kMxScaleTile;  // K may end inside the stage
         mbar_expect_tx(bar, S::kBBytes + S::kABytes + 2 * scale_bytes);
-        tma_load_2d(at, &tmap_b, bar, k * 128, n0);
-        tma_load_2d(at + S::kBBytes, &tmap_a, bar, k * 128, m0);
-        bulk_load_g2s(at + S::kBBytes + S::kABytes, sb + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
-        bulk_load_g2s(at + S::kBBytes + S::kABytes + kStepScales, sa + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
+        if (p.wide_boxes) {                                    // steps past the end of K read as zero
+          tma_load_3d(at, &tmap_b, bar, 0, n0, k);
+          tma_load_3d(at + S::kBBytes, &tmap_a, bar, 0, m0, k);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < kKPer; ++kk) {
+            tma_load_2d(at + kk * S::kBBlock, &tmap_b, bar, (k + kk) * 128, n0);
+            tma_load_2d(at + S::kBBytes + kk * S::kABlock, &tmap_a, bar, (k + kk) * 128, m0);
+          }
+        }
+        bulk_load_g2s(scales, sb + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
+        bulk_load_g2s(scales + S::kScaleBytes, sa + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
       }
       if (++stage == S::kStages) { stage = 0; phase ^= 1; }
     }
@@ -190,29 +208,42 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int k = k_first; k < k_last; ++k) {
+    for (int k = k_first; k < k_last; k += kKPer) {
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL));
       if (!ok) break;
       tc_fence_after();
       const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
-      const uint32_t scales = at + S::kBBytes + S::kABytes;
-      const uint32_t t_scales = tmem_base + kTN + stage * 16;  // 8 columns of B's scales, 8 of A's; free like the stage
-      const int mmas = min(kStepK, p.K - k * kStepK + kMmaK - 1) / kMmaK;
-      const uint64_t sdesc = make_scale_desc(scales);
+      const uint32_t t_scales = tmem_base + kTN + stage * 2 * S::kSetCols;  // B's scales, then A's; free like the stage
+      const int mmas = min(kKPer * kStepK, p.K - k * kStepK + kMmaK - 1) / kMmaK;
+      const uint64_t sdesc = make_scale_desc(at + S::kBBytes + S::kABytes);
       const uint64_t bdesc = make_kmajor_desc(at, 1024, 2);
       const uint64_t adesc = make_kmajor_desc(at + S::kBBytes, 1024, 2);
       if (elect_one()) {
+        constexpr int kPerStep = kStepK / kMmaK;
+        const auto copy = [&](int w) {
+          tmem_copy_scales<1>(t_scales + 4 * w, sdesc + w * (kMxScaleTile >> 4));
+          tmem_copy_scales<1>(t_scales + S::kSetCols + 4 * w, sdesc + ((S::kScaleBytes + w * kMxScaleTile) >> 4));
+        };
+        const auto product = [&](int i, bool accumulate) {
+          umma_mxf4<1>(tmem_base, bdesc + ((i / kPerStep) * (S::kBBlock >> 4) + 2 * (i % kPerStep)),
+                       adesc + ((i / kPerStep) * (S::kABlock >> 4) + 2 * (i % kPerStep)), make_idesc_mxf4(128, kTN, 2 * (i & 1)),
+                       t_scales + 4 * (i >> 1), t_scales + S::kSetCols + 4 * (i >> 1), accumulate);
+        };
+        if (mmas == kKPer * kPerStep) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
-          if (2 * w < mmas) {
-            tmem_copy_scales<1>(t_scales + 4 * w, sdesc + w * (kMxScaleTile >> 4));
-            tmem_copy_scales<1>(t_scales + 8 + 4 * w, sdesc + ((kStepScales + w * kMxScaleTile) >> 4));
-          }
+          for (int w = 0; w < 2 * kKPer; ++w) copy(w);
+          product(0, k > k_first);
 #pragma unroll
-        for (int i = 0; i < kStepK / kMmaK; ++i)
-          if (i < mmas)
-            umma_mxf4<1>(tmem_base, bdesc + 2 * i, adesc + 2 * i, make_idesc_mxf4(128, kTN, 2 * (i & 1)),
-                         t_scales + 4 * (i >> 1), t_scales + 8 + 4 * (i >> 1), (k > k_first || i > 0) ? 1u : 0u);
+          for (int i = 1; i < kKPer * kPerStep; ++i) product(i, true);
+        } else {
+#pragma unroll
+          for (int w = 0; w < 2 * kKPer; ++w)
+            if (2 * w < mmas) copy(w);
+          product(0, k > k_first);
+#pragma unroll
+          for (int i = 1; i < kKPer * kPerStep; ++i)
+            if (i < mmas) product(i, true);
+        }
         umma_commit(smem_u32(&empty_bar[stage]));
       }
       __syncwarp();
@@ -241,16 +272,25 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     }
   }
   tc_fence_before();
-  cluster_sync_all();  // every CTA's partial sums are in place (one CTA: a barrier over its warps)
+  if (split > 1) cluster_sync_all();  // every CTA's partial sums are in place
+  else __syncthreads();
 
   if (ok) {
     const int first = valid * rank / split, last = valid * (rank + 1) / split;
-    const uint32_t mine = smem_u32(partial) + lane * 16;
+    const float4* mine = reinterpret_cast<const float4*>(partial) + lane;
     for (int j = first + warp; j < last; j += 4) {
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int c = 0; c < split; ++c) {
-        const float4 o = ld_cluster_f4(mapa_u32(mine + j * 512, c));
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      float4 v;
+      if (split == 1) {
+        v = mine[j * 32];
+      } else {
+        float4 o[kMaxSplit];                           // all on their way before the first is added
+#pragma unroll
+        for (int c = 0; c < kMaxSplit; ++c)
+          if (c < split) o[c] = ld_cluster_f4(mapa_u32(smem_u32(mine + j * 32), c));
+        v = o[0];
+#pragma unroll
+        for (int c = 1; c < kMaxSplit; ++c)
+          if (c < split) { v.x += o[c].x; v.y += o[c].y; v.z += o[c].z; v.w += o[c].w; }
       }
       if constexpr (kOut == MX_MX) store_blocks(p, m0 + j, n0, lane, v);
       else if (n0 + 4 * lane < p.N) store4<kOut>(p, m0 + j, n0 + 4 * lane, v);
@@ -263,7 +303,7 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                                        mx_scale_word(m & 127)) = 0;
     }
   }
-  cluster_sync_all();  // the others may still read this CTA's partial sums
+  if (split > 1) cluster_sync_all();  // the others may still read this CTA's partial sums
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<1>(tmem_base, S::kTmemCols);
@@ -290,12 +330,30 @@ int encode_codes_map(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* codes, lo
   return AIEHLC_OK;
 }
 
+// Codes as a 3-D tensor {128 bytes, rows, K / 256}: one box brings `steps` steps of K.  K a multiple of 256.
+int encode_codes_map_3d(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* codes, long long rows, long long cols, int box_rows, int steps) {
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(cols / kStepK)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(mx_pitch(cols)), 128};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(steps)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(codes), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AIEHLC_ERR_CUDA, "cuTensorMapEncodeTiled (3-D) failed for the codes of a 4-bit operand");
+  return AIEHLC_OK;
+}
+
 template <int kTN, int kOut>
 int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStream_t st) {
   using S = NarrowShape<kTN>;
   CUtensorMap ma, mb;
-  if (int rc = encode_codes_map(ctx, &ma, c.A, c.M, c.K, kTN)) return rc;
-  if (int rc = encode_codes_map(ctx, &mb, c.B, c.N, c.K, 128)) return rc;
+  if (p.wide_boxes) {
+    if (int rc = encode_codes_map_3d(ctx, &ma, c.A, c.M, c.K, kTN, kKPer)) return rc;
+    if (int rc = encode_codes_map_3d(ctx, &mb, c.B, c.N, c.K, 128, kKPer)) return rc;
+  } else {
+    if (int rc = encode_codes_map(ctx, &ma, c.A, c.M, c.K, kTN)) return rc;
+    if (int rc = encode_codes_map(ctx, &mb, c.B, c.N, c.K, 128)) return rc;
+  }
   p.m_tiles = (c.M + kTN - 1) / kTN;
   p.n_tiles = (c.N + 127) / 128;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
@@ -303,7 +361,7 @@ int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStr
   KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
   if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::kTotal, &ks.smem_attr)) return rc;
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * ctx->usable_sms() && split * 4 <= p.k_steps) split *= 2;
+  while (split < kMaxSplit && tiles * split * 2 <= 2 * ctx->usable_sms() && split * 4 <= p.k_steps) split *= 2;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -320,19 +378,6 @@ int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStr
   cfg.numAttrs = ctx->pdl ? 2 : 1;
   AIEHLC_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, p));
   ctx->launches++;
-  return AIEHLC_OK;
-}
-
-// Codes as a 3-D tensor {128 bytes, rows, K / 256}: one box brings `steps` steps of K.  K a multiple of 256.
-int encode_codes_map_3d(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* codes, long long rows, long long cols, int box_rows, int steps) {
-  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(cols / kStepK)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(mx_pitch(cols)), 128};
-  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(steps)};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(codes), dims, strides, box, estr,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(AIEHLC_ERR_CUDA, "cuTensorMapEncodeTiled (3-D) failed for the codes of a 4-bit operand");
   return AIEHLC_OK;
 }
 
@@ -373,7 +418,6 @@ template <int kBN, int kOut>
 int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStream_t st) {
   using S = MxPairShape<kBN>;
   CUtensorMap ma, mb, mas, mbs, mc;
-  p.wide_boxes = c.K % kStepK == 0 && ctx->k_per_load != 1;
   if (p.wide_boxes) {
     if (int rc = encode_codes_map_3d(ctx, &ma, c.A, c.M, c.K, 128, kKPer)) return rc;
     if (int rc = encode_codes_map_3d(ctx, &mb, c.B, c.N, c.K, kBN / 2, kKPer)) return rc;
@@ -423,6 +467,7 @@ int launch_out(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
   p.M = c.M; p.N = c.N; p.K = c.K;
   p.k_steps = (c.K + kStepK - 1) / kStepK;
   p.words = static_cast<int>(mx_words(c.K));
+  p.wide_boxes = c.K % kStepK == 0 && ctx->k_per_load != 1;
   p.a_scales = c.As; p.b_scales = c.Bs;
   p.C = c.C; p.c_scales = c.Cs; p.ldc = c.ldc;
   const int esize = kOut == MX_F32 || kOut == MX_F32_ADD ? 4 : 2;

@@ -25,11 +25,8 @@ namespace aiehlc {
 namespace {
 
 constexpr int kMxPairThreads = 320;
-// Steps of K (256 elements each) per pipeline stage.  A commit costs the tensor cores' queue about 50 cycles (measured: 166
-// cycles per product with one commit per eight products, 179 with one more per four), so a stage is as long as
-// shared memory allows.
-constexpr int kKPer = 2;
-
+// A stage holds kKPer steps of K: a commit costs the tensor cores' queue about 50 cycles (measured: 166 cycles per product
+// with one commit per eight products, 179 with one more per four), so a stage is as long as shared memory allows.
 template <int kBN>
 struct MxPairShape {
   static constexpr int kABlock = 128 * 128;                    // 256 elements of K of this CTA's rows of A
@@ -213,12 +210,20 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           const int mmas = min(kKPer * kStepK, p.K - k * kStepK + kMmaK - 1) / kMmaK;
           if (elect_one()) {
             constexpr int kPerStep = kStepK / kMmaK;
+            const auto product = [&](int i, bool accumulate) {
+              umma_mxf4<2>(d_tmem, adesc + ((i / kPerStep) * (S::kABlock >> 4) + 2 * (i % kPerStep)),
+                           bdesc + ((i / kPerStep) * (S::kBBlock >> 4) + 2 * (i % kPerStep)), make_idesc_mxf4(256, kBN, 2 * (i & 1)),
+                           t_scales + (i >> 1) * S::kWordCols, t_scales + (i >> 1) * S::kWordCols + 4, accumulate);
+            };
+            product(0, k > 0);
+            if (mmas == kKPer * kPerStep) {   // straight through: a test per product costs the issuing thread 20 to 40 cycles
 #pragma unroll
-            for (int i = 0; i < kKPer * kPerStep; ++i)
-              if (i < mmas)
-                umma_mxf4<2>(d_tmem, adesc + ((i / kPerStep) * (S::kABlock >> 4) + 2 * (i % kPerStep)),
-                             bdesc + ((i / kPerStep) * (S::kBBlock >> 4) + 2 * (i % kPerStep)), make_idesc_mxf4(256, kBN, 2 * (i & 1)),
-                             t_scales + (i >> 1) * S::kWordCols, t_scales + (i >> 1) * S::kWordCols + 4, (k > 0 || i > 0) ? 1u : 0u);
+              for (int i = 1; i < kKPer * kPerStep; ++i) product(i, true);
+            } else {
+#pragma unroll
+              for (int i = 1; i < kKPer * kPerStep; ++i)
+                if (i < mmas) product(i, true);
+            }
             umma_commit_pair_mask(smem_u32(&empty_bar[stage]), 3);
           }
           __syncwarp();

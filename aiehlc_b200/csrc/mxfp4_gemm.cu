@@ -2,6 +2,8 @@
 //     C[m][n] = sum_k A[m][k] * B[n][k],  each factor an e2m1 number times its block's power of two.
 // The products are exact, the sums are held in 32 bits (TMEM).  C leaves as f32 (optionally added to what is there),
 // bf16, f16, or quantised again along its rows.
+#include <algorithm>
+
 #include "context.h"
 #include "mxfp4.cuh"
 #include "sm100_ptx.cuh"
@@ -27,11 +29,12 @@ struct MxGemmParams {
   void* C;                  // f32 / bf16 / f16, leading dimension ldc; MX_MX: codes
   uint8_t* c_scales;        // MX_MX
   long long ldc;
-  int vec_ok;               // four results at a time may be stored as a vector
+  int vec_ok;               // rows of C start on 16 bytes: vector stores
   int m_tiles, n_tiles;
+  int tile_store;           // CTA pairs: results leave as TMA tile stores
+  int stages;               // narrow form: stages in flight
   int group_m;              // CTA pairs: row blocks walked before the next column block
   int wide_boxes;           // one box brings all steps of a stage (K a multiple of 256)
-  int tile_store;           // CTA pairs: results leave as TMA tile stores
   int* status;
   int debug;                // 3: the producer withholds its loads, so every wait runs out
 };
@@ -45,7 +48,6 @@ struct MxGemmParams {
 // product with 16 columns takes 32), and with 256 elements they set the pace.
 template <int kTN>
 struct NarrowShape {
-  static constexpr int kStages = kTN == 128 ? 2 : 3;
   static constexpr int kBBlock = 128 * 128;                   // 256 elements of K of the tile's rows of B
   static constexpr int kABlock = kTN * 128;
   static constexpr int kBBytes = kBBlock * kKPer;
@@ -53,11 +55,13 @@ struct NarrowShape {
   static constexpr int kScaleBytes = kStepScales * kKPer;     // of each operand
   static constexpr int kStageBytes = kBBytes + kABytes + 2 * kScaleBytes;
   static constexpr int kPartialBytes = kTN * 128 * 4;         // over the stages, once they are done
-  static constexpr int kPool = kStages * kStageBytes > kPartialBytes ? kStages * kStageBytes : kPartialBytes;
-  static constexpr int kTotal = 1024 + kPool + 256;
+  static constexpr int kLimit = 227 * 1024 - 1024 - 256;
+  static constexpr int kMaxStages = kLimit / kStageBytes;     // 5, 5, 4, 3
+  static constexpr int pool(int stages) { return stages * kStageBytes > kPartialBytes ? stages * kStageBytes : kPartialBytes; }
+  static constexpr int total(int stages) { return 1024 + pool(stages) + 256; }
   static constexpr int kSetCols = 8 * kKPer;                  // columns of each operand's scales per stage
-  static constexpr int kScaleCols = 2 * kSetCols * kStages;
-  static constexpr int kTmemCols = kTN <= 32 ? 128 : 256;
+  static constexpr int kScaleCols = 2 * kSetCols * kMaxStages;
+  static constexpr int kTmemCols = 256;                       // two CTAs per SM at most
   static_assert(kTN + kScaleCols <= kTmemCols, "TMEM");
 };
 
@@ -133,9 +137,9 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   using S = NarrowShape<kTN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kPool);
-  uint64_t* empty_bar = full_bar + S::kStages;
-  uint64_t* done_bar = empty_bar + S::kStages;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::pool(p.stages));
+  uint64_t* empty_bar = full_bar + S::kMaxStages;
+  uint64_t* done_bar = empty_bar + S::kMaxStages;
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
 
@@ -151,7 +155,7 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   const int k_last = static_cast<int>(static_cast<long long>(k_stages) * (rank + 1) / split) * kKPer;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
@@ -200,7 +204,7 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         bulk_load_g2s(scales, sb + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
         bulk_load_g2s(scales + S::kScaleBytes, sa + static_cast<long long>(k) * kStepScales, scale_bytes, bar);
       }
-      if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
     if (!ok)
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land before the CTA retires
@@ -247,7 +251,7 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         umma_commit(smem_u32(&empty_bar[stage]));
       }
       __syncwarp();
-      if (++stage == S::kStages) { stage = 0; phase ^= 1; }
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
     if (ok && elect_one()) umma_commit(smem_u32(done_bar));
   }
@@ -359,9 +363,20 @@ int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStr
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
   auto kern = mx_gemm_narrow_kernel<kTN, kOut>;
   KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
-  if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::kTotal, &ks.smem_attr)) return rc;
+  // Up to one CTA per SM: K is split over as many CTAs as there are SMs for (each with two stages to do; with 128 columns, where
+  // a stage takes longer, one), and the ring is as deep as shared memory allows.  More tiles than that: two CTAs
+  // share an SM, with a ring of two stages each.
+  const int sms = ctx->usable_sms(), k_stages = (p.k_steps + kKPer - 1) / kKPer;
   int split = 1;
-  while (split < kMaxSplit && tiles * split * 2 <= 2 * ctx->usable_sms() && split * 4 <= p.k_steps) split *= 2;
+  p.stages = S::kMaxStages;
+  if (tiles <= sms) {
+    split = std::min(static_cast<int>(sms / tiles), kTN == 128 ? k_stages : k_stages / 2);
+    split = std::max(1, std::min(split, kMaxSplit));
+  } else if (2 * S::total(2) <= 226 * 1024) {
+    p.stages = 2;
+  }
+  const int smem_bytes = S::total(p.stages);
+  if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::total(S::kMaxStages), &ks.smem_attr)) return rc;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -372,7 +387,7 @@ int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStr
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
   cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = S::kTotal;
+  cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = ctx->pdl ? 2 : 1;
@@ -395,11 +410,11 @@ int encode_scales_map(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* scales, 
   return AIEHLC_OK;
 }
 
-// C as the output warps store it: 32 rows x 128 bytes (codes of a kBN-column tile: kBN / 2 bytes).
+// C as the output warps of a CTA pair store it: 32 rows x 64 bytes (codes: all kBN / 2 bytes of the tile's rows).
 template <int kBN, int kOut>
 int encode_result_map(aiehlc_ctx* ctx, CUtensorMap* map, const MxGemmCall& c) {
   constexpr int esize = kOut == MX_MX ? 1 : kOut == MX_F32 || kOut == MX_F32_ADD ? 4 : 2;
-  constexpr int row_bytes = kOut == MX_MX ? kBN / 2 : 128;
+  constexpr int row_bytes = kOut == MX_MX ? kBN / 2 : 64;
   const long long cols = kOut == MX_MX ? mx_pitch(c.N) : c.N;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(c.M)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(kOut == MX_MX ? cols : c.ldc * esize)};
@@ -471,7 +486,7 @@ int launch_out(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
   p.a_scales = c.As; p.b_scales = c.Bs;
   p.C = c.C; p.c_scales = c.Cs; p.ldc = c.ldc;
   const int esize = kOut == MX_F32 || kOut == MX_F32_ADD ? 4 : 2;
-  p.vec_ok = reinterpret_cast<uintptr_t>(c.C) % (4 * esize) == 0 && c.ldc % 4 == 0;
+  p.vec_ok = reinterpret_cast<uintptr_t>(c.C) % 16 == 0 && c.ldc * esize % 16 == 0;
   p.status = ctx->d_status;
   p.debug = ctx->debug_mode;
   if (c.M > 128 || ctx->pair_mode == 1) {

@@ -340,44 +340,37 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             else words[0] |= byte;
           }
         } else if (kOut != MX_F32_ADD && p.tile_store) {
-          if constexpr (kOut == MX_F32) {
+          // 64-byte pieces of 32 rows, through the two halves of this warp's buffer in turn
+          constexpr int kCols = kOut == MX_F32 ? 16 : 32;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (lane == 0) tma_store_wait_read<0>();
-              __syncwarp();
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ swz) << 4)) = make_uint4(r[h][4 * j], r[h][4 * j + 1], r[h][4 * j + 2], r[h][4 * j + 3]);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_2d(&tmap_c, smem_u32(buf), n0 + c + 32 * h, row0);
-                tma_store_commit();
-              }
-            }
-          } else {
-            if (lane == 0) tma_store_wait_read<0>();
+          for (int h = 0; h < 64 / kCols; ++h) {
+            uint8_t* piece = buf + (h & 1) * 2048;
+            if (lane == 0) tma_store_wait_read<1>();   // the store before the last has read it
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
               uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float lo = __uint_as_float(r[j >> 2][8 * (j & 3) + 2 * i]), hi = __uint_as_float(r[j >> 2][8 * (j & 3) + 2 * i + 1]);
-                if constexpr (kOut == MX_BF16) {
-                  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-                  w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                if constexpr (kOut == MX_F32) {
+                  w[i] = r[h >> 1][16 * (h & 1) + 4 * j + i];
                 } else {
-                  const __half2 v = __floats2half2_rn(lo, hi);
-                  w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                  const float lo = __uint_as_float(r[h][8 * j + 2 * i]), hi = __uint_as_float(r[h][8 * j + 2 * i + 1]);
+                  if constexpr (kOut == MX_BF16) {
+                    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                  } else {
+                    const __half2 v = __floats2half2_rn(lo, hi);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                  }
                 }
               }
-              *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ swz) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(piece + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&tmap_c, smem_u32(buf), n0 + c, row0);
+              tma_store_2d(&tmap_c, smem_u32(piece), n0 + c + kCols * h, row0);
               tma_store_commit();
             }
           }

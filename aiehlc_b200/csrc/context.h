@@ -50,6 +50,7 @@ namespace aiehlc {
 struct KernelSetup {
   int smem_attr = 0;     // dynamic shared memory limit already raised to this many bytes
   int max_clusters = 0;  // co-resident clusters of the persistent pair kernel (0 = not queried)
+  int clusters_of[9] = {};  // narrow 4-bit products: co-resident clusters of 1 .. 8 CTAs (0 = not queried)
 };
 }  // namespace aiehlc
 

@@ -31,6 +31,7 @@ struct MxGemmParams {
   long long ldc;
   int vec_ok;               // rows of C start on 16 bytes: vector stores
   int m_tiles, n_tiles;
+  int tail_first;           // CTA pairs: tiles from this one on run as two column halves each (the number of tiles: none do)
   int tile_store;           // CTA pairs: results leave as TMA tile stores
   int stages;               // narrow form: stages in flight
   int group_m;              // CTA pairs: row blocks walked before the next column block
@@ -129,6 +130,39 @@ __device__ __forceinline__ void store_blocks(const MxGemmParams& p, int m, int n
   if (lane == 0)
     *reinterpret_cast<uint32_t*>(p.c_scales + (static_cast<long long>(m / 128) * mx_words(p.N) + n0 / 128) * kMxScaleTile +
                                  mx_scale_word(m & 127)) = word;
+}
+
+// Adds the cluster's partial sums of rows first .. last - 1 of the tile (those of one row by one warp, four columns a lane, in
+// the order of the ranks) and sends them through the output stage.  A read of another CTA's shared memory takes most of a
+// microsecond, so kRows rows of up to kSplit shares are on their way together: 16 reads a thread.
+template <int kRows, int kSplit, int kOut>
+__device__ __forceinline__ void sum_rows(const MxGemmParams& p, const float* partial, int split, int first, int last, int m0, int n0) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t mine = smem_u32(partial) + lane * 16;
+  for (int j0 = first + warp; j0 < last; j0 += 4 * kRows) {
+    float4 o[kRows][kSplit];
+#pragma unroll
+    for (int c = 0; c < kSplit; ++c) {
+      if (c < split) {
+        const uint32_t at = mapa_u32(mine, c);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (j0 + 4 * i < last) o[i][c] = ld_cluster_f4(at + (j0 + 4 * i) * 512);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int j = j0 + 4 * i;
+      if (j < last) {
+        float4 v = o[i][0];
+#pragma unroll
+        for (int c = 1; c < kSplit; ++c)
+          if (c < split) { v.x += o[i][c].x; v.y += o[i][c].y; v.z += o[i][c].z; v.w += o[i][c].w; }
+        if constexpr (kOut == MX_MX) store_blocks(p, m0 + j, n0, lane, v);
+        else if (n0 + 4 * lane < p.N) store4<kOut>(p, m0 + j, n0 + 4 * lane, v);
+      }
+    }
+  }
 }
 
 template <int kTN, int kOut>
@@ -281,24 +315,9 @@ mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 
   if (ok) {
     const int first = valid * rank / split, last = valid * (rank + 1) / split;
-    const float4* mine = reinterpret_cast<const float4*>(partial) + lane;
-    for (int j = first + warp; j < last; j += 4) {
-      float4 v;
-      if (split == 1) {
-        v = mine[j * 32];
-      } else {
-        float4 o[kMaxSplit];                           // all on their way before the first is added
-#pragma unroll
-        for (int c = 0; c < kMaxSplit; ++c)
-          if (c < split) o[c] = ld_cluster_f4(mapa_u32(smem_u32(mine + j * 32), c));
-        v = o[0];
-#pragma unroll
-        for (int c = 1; c < kMaxSplit; ++c)
-          if (c < split) { v.x += o[c].x; v.y += o[c].y; v.z += o[c].z; v.w += o[c].w; }
-      }
-      if constexpr (kOut == MX_MX) store_blocks(p, m0 + j, n0, lane, v);
-      else if (n0 + 4 * lane < p.N) store4<kOut>(p, m0 + j, n0 + 4 * lane, v);
-    }
+    if (split <= 2) sum_rows<8, 2, kOut>(p, partial, split, first, last, m0, n0);
+    else if (split <= 4) sum_rows<4, 4, kOut>(p, partial, split, first, last, m0, n0);
+    else sum_rows<2, kMaxSplit, kOut>(p, partial, split, first, last, m0, n0);
     if constexpr (kOut == MX_MX) {
       // rows of the last scale tile that do not exist
       if (rank == 0 && m0 + kTN >= p.M)
@@ -347,6 +366,43 @@ int encode_codes_map_3d(aiehlc_ctx* ctx, CUtensorMap* map, const uint8_t* codes,
   return AIEHLC_OK;
 }
 
+// How many CTAs share the K of a tile of the narrow form: as many as there are SMs for with one CTA on each, all clusters
+// resident at once (clusters do not straddle GPCs, so fewer large ones fit than the SM count says: 128 CTAs ran in 5.2 us as
+// clusters of four and in 11.8 us, two waves, as clusters of eight), and each CTA with two stages to do (with 128 columns, where a
+// stage takes longer, one).
+template <int kTN, int kOut>
+int narrow_split(aiehlc_ctx* ctx, long long tiles, int k_stages) {
+  using S = NarrowShape<kTN>;
+  const int sms = ctx->usable_sms();
+  if (tiles > sms) return 1;
+  auto kern = mx_gemm_narrow_kernel<kTN, kOut>;
+  KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
+  int split = std::min(static_cast<int>(sms / tiles), kTN == 128 ? k_stages : k_stages / 2);
+  for (split = std::min(split, kMaxSplit); split > 1; --split) {
+    int& fit = ks.clusters_of[split];
+    if (fit == 0) {
+      cudaLaunchConfig_t cfg{};
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = split;
+      attr.val.clusterDim.y = 1;
+      attr.val.clusterDim.z = 1;
+      cfg.gridDim = dim3(split);
+      cfg.blockDim = dim3(128);
+      cfg.dynamicSmemBytes = S::total(S::kMaxStages);
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::total(S::kMaxStages), &ks.smem_attr)) return 1;
+      if (cudaOccupancyMaxActiveClusters(&fit, kern, &cfg) != cudaSuccess || fit <= 0) {
+        cudaGetLastError();
+        fit = -1;
+      }
+    }
+    if (tiles <= fit) return split;
+  }
+  return 1;
+}
+
 template <int kTN, int kOut>
 int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStream_t st) {
   using S = NarrowShape<kTN>;
@@ -363,18 +419,9 @@ int launch_narrow(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStr
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
   auto kern = mx_gemm_narrow_kernel<kTN, kOut>;
   KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
-  // Up to one CTA per SM: K is split over as many CTAs as there are SMs for (each with two stages to do; with 128 columns, where
-  // a stage takes longer, one), and the ring is as deep as shared memory allows.  More tiles than that: two CTAs
-  // share an SM, with a ring of two stages each.
-  const int sms = ctx->usable_sms(), k_stages = (p.k_steps + kKPer - 1) / kKPer;
-  int split = 1;
-  p.stages = S::kMaxStages;
-  if (tiles <= sms) {
-    split = std::min(static_cast<int>(sms / tiles), kTN == 128 ? k_stages : k_stages / 2);
-    split = std::max(1, std::min(split, kMaxSplit));
-  } else if (2 * S::total(2) <= 226 * 1024) {
-    p.stages = 2;
-  }
+  // One CTA per SM has a ring as deep as shared memory allows; with more tiles than SMs two share one, with two stages each.
+  const int split = narrow_split<kTN, kOut>(ctx, tiles, (p.k_steps + kKPer - 1) / kKPer);
+  p.stages = tiles > ctx->usable_sms() && 2 * S::total(2) <= 226 * 1024 ? 2 : S::kMaxStages;
   const int smem_bytes = S::total(p.stages);
   if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::total(S::kMaxStages), &ks.smem_attr)) return rc;
   cudaLaunchConfig_t cfg{};
@@ -432,7 +479,7 @@ int encode_result_map(aiehlc_ctx* ctx, CUtensorMap* map, const MxGemmCall& c) {
 template <int kBN, int kOut>
 int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStream_t st) {
   using S = MxPairShape<kBN>;
-  CUtensorMap ma, mb, mas, mbs, mc;
+  CUtensorMap ma, mb, mbh, mas, mbs, mc;
   if (p.wide_boxes) {
     if (int rc = encode_codes_map_3d(ctx, &ma, c.A, c.M, c.K, 128, kKPer)) return rc;
     if (int rc = encode_codes_map_3d(ctx, &mb, c.B, c.N, c.K, kBN / 2, kKPer)) return rc;
@@ -452,7 +499,18 @@ int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStrea
   p.m_tiles = (c.M + 255) / 256;
   p.n_tiles = (c.N + kBN - 1) / kBN;
   p.group_m = ctx->group_m > 0 ? ctx->group_m : 8;
-  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  const int tiles = p.m_tiles * p.n_tiles;
+  const int limit = ctx->usable_sms() / 2 > 0 ? ctx->usable_sms() / 2 : 1;
+  // A last wave that keeps at most half of the pairs busy: its tiles are cut into two column halves that run side by side
+  int parts = 1;
+  narrow_tail(tiles, limit, kBN, tiles > limit ? ctx->split_tail : 0, &p.tail_first, &parts);
+  mbh = mb;
+  if (parts == 2) {
+    if (p.wide_boxes) {
+      if (int rc = encode_codes_map_3d(ctx, &mbh, c.B, c.N, c.K, kBN / 4, kKPer)) return rc;
+    } else if (int rc = encode_codes_map(ctx, &mbh, c.B, c.N, c.K, kBN / 4)) return rc;
+  }
+  const int units = 2 * tiles - p.tail_first;
   auto kern = mx_gemm_pair_kernel<kBN, kOut>;
   KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
   if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), S::kTotal, &ks.smem_attr)) return rc;
@@ -464,14 +522,13 @@ int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStrea
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
-  const long long limit = ctx->usable_sms() / 2 > 0 ? ctx->usable_sms() / 2 : 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < limit ? tiles : limit)));
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min(units, limit)));
   cfg.blockDim = dim3(kMxPairThreads);
   cfg.dynamicSmemBytes = S::kTotal;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = ctx->pdl ? 2 : 1;
-  AIEHLC_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, mas, mbs, mc, p));
+  AIEHLC_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, mbh, mas, mbs, mc, p));
   ctx->launches++;
   return AIEHLC_OK;
 }
@@ -489,10 +546,21 @@ int launch_out(aiehlc_ctx* ctx, const MxGemmCall& c, cudaStream_t st) {
   p.vec_ok = reinterpret_cast<uintptr_t>(c.C) % 16 == 0 && c.ldc * esize % 16 == 0;
   p.status = ctx->d_status;
   p.debug = ctx->debug_mode;
-  if (c.M > 128 || ctx->pair_mode == 1) {
+  // Up to 64 rows of A: the narrow form.  More: CTA pairs, unless there are so few tiles that most SMs would be idle and K is
+  // long enough for splitting it to pay (narrow form, 128 columns).  Measured, us, narrow / pairs: 128 x 4096 x 1024 7.1 / 5.0,
+  // 128 x 4096 x 4096 8.4 / 7.5, 128 x 8192 x 8192 11.5 / 11.7, 128 x 512 x 16384 8.4 / 16.4, 67 x 1001 x 4103 6.9 / 7.9:
+  // about 0.41 us per stage for a wave of pairs, 0.5 for a narrow CTA, and 2.7 us for joining the partial sums.
+  const int sms = ctx->usable_sms(), k_stages = (p.k_steps + kKPer - 1) / kKPer;
+  bool pairs = ctx->pair_mode == 1 || (ctx->pair_mode != 0 && c.M > 64 && sms >= 2);
+  if (pairs && ctx->pair_mode != 1) {
+    const long long tiles = ((c.M + 127LL) / 128) * ((c.N + 127LL) / 128);
+    const int split = narrow_split<128, kOut>(ctx, tiles, k_stages);
+    if (split > 1 && 0.41 * k_stages > 0.5 * k_stages / split + 2.7) pairs = false;
+  }
+  if (pairs) {
+    // half as wide tiles where that at least doubles the SMs at work
     const long long tiles = ((c.M + 255LL) / 256) * ((c.N + 255LL) / 256);
-    if (ctx->force_tile_n == 128 || (ctx->force_tile_n == 0 && tiles * 2 <= ctx->usable_sms() / 2))
-      return launch_pair<128, kOut>(ctx, c, p, st);
+    if (ctx->force_tile_n == 128 || (ctx->force_tile_n == 0 && tiles * 2 <= sms / 2)) return launch_pair<128, kOut>(ctx, c, p, st);
     return launch_pair<256, kOut>(ctx, c, p, st);
   }
   if (c.M <= 16) return launch_narrow<16, kOut>(ctx, c, p, st);

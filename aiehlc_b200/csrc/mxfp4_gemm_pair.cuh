@@ -52,8 +52,15 @@ struct MxPairShape {
   static_assert(kStageBytes % 1024 == 0 && kScaleCol + kSets * kSetCols <= kTmemCols && kSets <= kStages, "layout");
 };
 
-// Tiles walk group_m row blocks before the next column block.
-__device__ __forceinline__ void mx_tile(const MxGemmParams& p, int t, int& mb, int& nb) {
+// Unit `u` of the launch: a tile, or (thin last wave: p.tail_first) one of the two column halves of a tail tile.  Tiles walk
+// group_m row blocks before the next column block.
+__device__ __forceinline__ void mx_unit(const MxGemmParams& p, int u, int& mb, int& nb, int& part) {
+  int t = u;
+  part = -1;
+  if (u >= p.tail_first) {
+    t = p.tail_first + ((u - p.tail_first) >> 1);
+    part = (u - p.tail_first) & 1;
+  }
   const int per_group = p.group_m * p.n_tiles;
   const int g = t / per_group;
   const int first = g * p.group_m;
@@ -85,7 +92,7 @@ __device__ __forceinline__ void store_rows(const MxGemmParams& p, uint8_t* buf, 
 template <int kBN, int kOut>
 __global__ void __launch_bounds__(kMxPairThreads, 1)
 mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                    const __grid_constant__ CUtensorMap tmap_as, const __grid_constant__ CUtensorMap tmap_bs,
+                    const __grid_constant__ CUtensorMap tmap_b_half, const __grid_constant__ CUtensorMap tmap_as, const __grid_constant__ CUtensorMap tmap_bs,
                     const __grid_constant__ CUtensorMap tmap_c, const MxGemmParams p) {
   using S = MxPairShape<kBN>;
   constexpr int kStages = S::kStages;
@@ -138,41 +145,45 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   pdl_launch_dependents();
   pdl_wait();
   const int num_tiles = p.m_tiles * p.n_tiles;
+  const int num_units = 2 * num_tiles - p.tail_first;
 
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair_id; ok && t < num_tiles; t += num_pairs) {
-        int mb, nb;
-        mx_tile(p, t, mb, nb);
+      for (int t = pair_id; ok && t < num_units; t += num_pairs) {
+        int mb, nb, part;
+        mx_unit(p, t, mb, nb, part);
+        const int b_rows = kBN / (part < 0 ? 2 : 4);
+        const int row_b = nb * kBN + (part > 0 ? kBN / 2 : 0) + rank * b_rows;
+        const int scales_b = nb * S::kBTiles + (part > 0 ? S::kBTiles / 2 : 0);
+        const CUtensorMap* map_b = part < 0 ? &tmap_b : &tmap_b_half;
         for (int k = 0; k < p.k_steps; k += kKPer) {
           ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status, ST_TIMEOUT_EMPTY);
           if (!ok) break;
           if (p.debug != 3) {
-            if (leader) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * (S::kABytes + S::kBBytes));
+            if (leader) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * (S::kABytes + kKPer * 128 * b_rows));
             const uint32_t bar = mapa_u32(smem_u32(&full_bar[stage]), 0);
             const uint32_t sa = smem_u32(smem + stage * S::kStageBytes);
             const uint32_t sb = sa + S::kABytes;
             const uint32_t ss = sb + S::kBBytes;
             const int row_a = mb * 256 + rank * 128;
-            const int row_b = nb * kBN + rank * (kBN / 2);
             // steps past the end of K read as zero
             if (p.wide_boxes) {
               tma_load_3d_pair(sa, &tmap_a, bar, 0, row_a, k);
-              tma_load_3d_pair(sb, &tmap_b, bar, 0, row_b, k);
+              tma_load_3d_pair(sb, map_b, bar, 0, row_b, k);
             } else {
 #pragma unroll
               for (int kk = 0; kk < kKPer; ++kk) {
                 tma_load_2d_pair(sa + kk * S::kABlock, &tmap_a, bar, (k + kk) * 128, row_a);
-                tma_load_2d_pair(sb + kk * S::kBBlock, &tmap_b, bar, (k + kk) * 128, row_b);
+                tma_load_2d_pair(sb + kk * 128 * b_rows, map_b, bar, (k + kk) * 128, row_b);
               }
             }
             const uint32_t scales_bar = smem_u32(&scales_full_bar[stage]);
             mbar_expect_tx(scales_bar, S::kAScales + S::kBScales);
             tma_load_2d(ss, &tmap_as, scales_bar, k * (kStepScales / 8), mb * 2 + rank);
-            tma_load_2d(ss + S::kAScales, &tmap_bs, scales_bar, k * (kStepScales / 8), nb * S::kBTiles);
+            tma_load_2d(ss + S::kAScales, &tmap_bs, scales_bar, k * (kStepScales / 8), scales_b);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
@@ -188,7 +199,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       uint32_t set_phase = 0;
       int it = 0;
       bool ok = true;
-      for (int t = pair_id; ok && t < num_tiles; t += num_pairs, ++it) {
+      for (int t = pair_id; ok && t < num_units; t += num_pairs, ++it) {
         // The output stage has drained the accumulator's tile before this one.  Where the accumulators share columns, what
         // it signals is that it has read the shared ones of the last tile, for which it was through with the tile before.
         if constexpr (S::kShared) ok = it == 0 || mbar_wait(smem_u32(tmem_free_bar), (it - 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
@@ -197,6 +208,9 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (it & 1) * S::kAcc1;
+        const bool halved = t >= p.tail_first;
+        const uint32_t idesc = halved ? make_idesc_mxf4(256, kBN / 2, 0) : make_idesc_mxf4(256, kBN, 0);
+        const uint32_t b_block = S::kBBlock >> (halved ? 5 : 4);   // descriptor units from one step of K to the next
         for (int k = 0; k < p.k_steps; k += kKPer) {
           ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL) &&
                mbar_wait(smem_u32(&scales_set_bar[set]), set_phase, abort_flag, p.status, ST_TIMEOUT_FULL);
@@ -212,7 +226,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             constexpr int kPerStep = kStepK / kMmaK;
             const auto product = [&](int i, bool accumulate) {
               umma_mxf4<2>(d_tmem, adesc + ((i / kPerStep) * (S::kABlock >> 4) + 2 * (i % kPerStep)),
-                           bdesc + ((i / kPerStep) * (S::kBBlock >> 4) + 2 * (i % kPerStep)), make_idesc_mxf4(256, kBN, 2 * (i & 1)),
+                           bdesc + ((i / kPerStep) * b_block + 2 * (i % kPerStep)), idesc | make_idesc_mxf4_scale(2 * (i & 1)),
                            t_scales + (i >> 1) * S::kWordCols, t_scales + (i >> 1) * S::kWordCols + 4, accumulate);
             };
             product(0, k > 0);
@@ -243,7 +257,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     uint32_t phase = 0, old_phase = 0;
     long long used = 0;
     bool ok = true;
-    for (int t = pair_id; ok && t < num_tiles; t += num_pairs) {
+    for (int t = pair_id; ok && t < num_units; t += num_pairs) {
       for (int k = 0; k < p.k_steps; k += kKPer) {
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&scales_full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL));
         if (!ok) break;
@@ -279,22 +293,23 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     uint8_t* buf = staging + quad * 4096;
     const int swz = lane & 7;
     int it = 0;
-    for (int t = pair_id; t < num_tiles; t += num_pairs, ++it) {
-      int mb, nb;
-      mx_tile(p, t, mb, nb);
+    for (int t = pair_id; t < num_units; t += num_pairs, ++it) {
+      int mb, nb, part;
+      mx_unit(p, t, mb, nb, part);
       const int acc = it & 1;
       bool ok = mbar_wait(smem_u32(&tmem_full_bar[acc]), (it >> 1) & 1, abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       tc_fence_after();
       const int row0 = mb * 256 + rank * 128 + quad * 32;
-      const int n0 = nb * kBN;
+      const int n0 = nb * kBN + (part > 0 ? kBN / 2 : 0);
+      const int halves = part < 0 ? kBN / 128 : 1;   // a column half of a 256-column tile is 128 columns
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::kAcc1;
       uint32_t words[kBN / 128] = {};                  // MX_MX: this row's scales
 #pragma unroll 1
-      for (int half = 0; half < kBN / 128; ++half) {
+      for (int half = 0; half < halves; ++half) {
         // accumulator 0 of 256 columns shares its last ones, accumulator 1 its first
-        const int c_half = S::kShared && acc == 0 ? 128 - 128 * half : 128 * half;
+        const int c_half = S::kShared && acc == 0 && part < 0 ? 128 - 128 * half : 128 * half;
         uint32_t all[4][32];
         __syncwarp();
 #pragma unroll
@@ -334,7 +349,12 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
               w[g] = s == kMxNan ? 0 : mx_codes8(f);
             }
             const int piece = c / 32 + h;              // 16 bytes of codes per block
-            *reinterpret_cast<uint4*>(buf + lane * (kBN / 2) + ((piece ^ (kBN == 256 ? swz : (lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (part >= 0) {                           // a column half is not the tile store's box
+              if (row0 + lane < p.M && n < p.N)
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.C) + (static_cast<long long>(row0 + lane) * mx_pitch(p.N) + n / 2)) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+            } else
+              *reinterpret_cast<uint4*>(buf + lane * (kBN / 2) + ((piece ^ (kBN == 256 ? swz : (lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             const uint32_t byte = row0 + lane < p.M && n < p.N ? static_cast<uint32_t>(s) << (8 * (piece & 3)) : 0u;
             if (kBN == 256 && piece >= 4) words[kBN / 128 - 1] |= byte;
             else words[0] |= byte;
@@ -383,7 +403,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       if constexpr (kOut == MX_MX) {
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
+        if (lane == 0 && part < 0) {
           tma_store_2d(&tmap_c, smem_u32(buf), n0 / 2, row0);
           tma_store_commit();
         }
@@ -392,7 +412,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         if (row0 / 128 < (p.M + 127) / 128) {
 #pragma unroll
           for (int w = 0; w < kBN / 128; ++w)
-            if (n0 / 128 + w < c_words)
+            if (w < halves && n0 / 128 + w < c_words)
               *reinterpret_cast<uint32_t*>(p.c_scales + (static_cast<long long>(row0 / 128) * c_words + n0 / 128 + w) * kMxScaleTile +
                                            mx_scale_word((row0 + lane) & 127)) = words[w];
         }

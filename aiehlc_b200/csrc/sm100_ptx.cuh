@@ -419,9 +419,12 @@ __device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
 }
 // Instruction descriptor of kind::mxf4 (dense, K-major): bits [4,6) scale data id of B, [7,10) and [10,12) e2m1 operands,
 // [17,23) N >> 3, bit 23 power-of-two scales, [27,29) M >> 7, [29,31) scale data id of A.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4_scale(int id) {
+  return (static_cast<uint32_t>(id) << 4) | (static_cast<uint32_t>(id) << 29);
+}
 __host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int scale_id) {
-  return (static_cast<uint32_t>(scale_id) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(scale_id) << 29);
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27) |
+         make_idesc_mxf4_scale(scale_id);
 }
 
 // Instruction descriptor (dense, K-major A and B):

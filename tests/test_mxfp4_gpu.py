@@ -125,7 +125,10 @@ def test_dequantize_every_scale_and_code(ctx, kind):
 # ---------------------------------------------------------------- products
 SHAPES = [(1, 1, 1), (1, 16, 32), (2, 33, 31), (16, 128, 64), (17, 100, 33), (32, 130, 256), (33, 257, 500), (64, 96, 1000),
           (65, 129, 300), (100, 1000, 96), (128, 128, 2048), (129, 300, 4103), (256, 256, 512), (257, 513, 1030), (300, 700, 2049),
-          (520, 1000, 288), (1, 4096, 4096)]
+          (520, 1000, 288), (1, 4096, 4096),
+          # more tiles than CTA pairs: both accumulators in turn, a last wave of column halves; long K on few tiles; many
+          # narrow tiles, two to an SM
+          (2500, 2000, 300), (1300, 4500, 1030), (100, 200, 9000), (20, 30000, 1030)]
 
 
 def _bound(a, b, K, kind):

@@ -70,21 +70,61 @@ __device__ __forceinline__ void mx_unit(const MxGemmParams& p, int u, int& mb, i
   nb = r / rows;
 }
 
-// 32 rows x 32 columns of C, one row per lane, through this warp's staging buffer: out in whole 128-byte (f32) or
-// 64-byte row pieces, where C does not allow tile stores or is added to.
+// 32 rows x 32 columns of C, one row per lane, through this warp's staging buffer and out along the rows: where C does not
+// allow tile stores or is added to.  Rows that start on 16 bytes leave four columns a lane, others one column a lane, so
+// that a warp always stores neighbours; what is added to is read before anything is written.
 template <int kOut>
 __device__ __forceinline__ void store_rows(const MxGemmParams& p, uint8_t* buf, const uint32_t (&r)[32], int row0, int col0, int lane) {
+  const int swz = lane & 7;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ swz) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
   __syncwarp();
-  const int piece = lane & 7;
-  const int n = col0 + piece * 4;
+  constexpr int kBatch = 4;                            // reads on their way together
+  if (p.vec_ok) {
+    const int piece = lane & 7;
+    const int n = col0 + piece * 4;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 8; i0 += kBatch) {
+      float4 v[kBatch];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int at = i * 4 + (lane >> 3);
-    const float4 v = *reinterpret_cast<const float4*>(buf + at * 128 + ((piece ^ (at & 7)) << 4));
-    if (row0 + at < p.M && n < p.N) store4<kOut>(p, row0 + at, n, v);
+      for (int i = 0; i < kBatch; ++i) {
+        const int at = (i0 + i) * 4 + (lane >> 3);
+        v[i] = *reinterpret_cast<const float4*>(buf + at * 128 + ((piece ^ (at & 7)) << 4));
+        if (kOut == MX_F32_ADD && n + 4 <= p.N && row0 + at < p.M) {
+          const float4 was = *reinterpret_cast<const float4*>(static_cast<const float*>(p.C) + static_cast<long long>(row0 + at) * p.ldc + n);
+          v[i].x += was.x; v[i].y += was.y; v[i].z += was.z; v[i].w += was.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int at = (i0 + i) * 4 + (lane >> 3);
+        if (row0 + at < p.M && n < p.N) {
+          if (kOut == MX_F32_ADD && n + 4 <= p.N) store4<MX_F32>(p, row0 + at, n, v[i]);
+          else store4<kOut>(p, row0 + at, n, v[i]);
+        }
+      }
+    }
+  } else {
+    const int n = col0 + lane;
+    const int rows = n < p.N ? min(32, p.M - row0) : 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < rows; i0 += 2 * kBatch) {
+      const long long at = static_cast<long long>(row0 + i0) * p.ldc + n;
+      float v[2 * kBatch];
+#pragma unroll
+      for (int i = 0; i < 2 * kBatch; ++i) {
+        v[i] = *reinterpret_cast<const float*>(buf + (i0 + i) * 128 + ((((lane >> 2) ^ (i & 7)) << 4) | ((lane & 3) << 2)));
+        if (kOut == MX_F32_ADD && i0 + i < rows) v[i] += static_cast<const float*>(p.C)[at + i * p.ldc];
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * kBatch; ++i)
+        if (i0 + i < rows) {
+          if constexpr (kOut == MX_F32 || kOut == MX_F32_ADD) static_cast<float*>(p.C)[at + i * p.ldc] = v[i];
+          else if constexpr (kOut == MX_BF16) static_cast<__nv_bfloat16*>(p.C)[at + i * p.ldc] = __float2bfloat16_rn(v[i]);
+          else static_cast<__half*>(p.C)[at + i * p.ldc] = __float2half_rn(v[i]);
+        }
+    }
   }
   __syncwarp();
 }

@@ -3,6 +3,7 @@
 // The products are exact, the sums are held in 32 bits (TMEM).  C leaves as f32 (optionally added to what is there),
 // bf16, f16, or quantised again along its rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "context.h"
 #include "mxfp4.cuh"
@@ -491,8 +492,7 @@ int launch_pair(aiehlc_ctx* ctx, const MxGemmCall& c, MxGemmParams& p, cudaStrea
   if (int rc = encode_scales_map(ctx, &mbs, c.Bs, c.N, c.K, S::kBTiles, kKPer)) return rc;
   constexpr int esize = kOut == MX_F32 || kOut == MX_F32_ADD ? 4 : 2;
   // a tile store is clipped at the tensor's edge in pieces of 16 bytes: a row that ends inside one would be written past its end
-  p.tile_store = kOut == MX_MX || (kOut != MX_F32_ADD && reinterpret_cast<uintptr_t>(c.C) % 16 == 0 && c.ldc * esize % 16 == 0 &&
-                                   static_cast<long long>(c.N) * esize % 16 == 0);
+  p.tile_store = kOut == MX_MX || (reinterpret_cast<uintptr_t>(c.C) % 16 == 0 && c.ldc * esize % 16 == 0 && static_cast<long long>(c.N) * esize % 16 == 0);
   mc = ma;  // unused without tile stores
   if (p.tile_store)
     if (int rc = encode_result_map<kBN, kOut>(ctx, &mc, c)) return rc;

@@ -253,8 +253,9 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
 }
 
 // Values of a quantised matrix.  Bound by memory: 17/32 byte read, sizeof(T) written per element.  A CTA takes the
-// 128 x 128 elements of one scale tile; a thread turns four bytes of codes into eight values.  Where rows of y do not start
-// on 16 bytes (kVec false) a warp's two rows turn through shared memory, so that neighbouring lanes store neighbours.
+// 128 x 128 elements of one scale tile; a thread turns four bytes of codes into eight values.  f32 values, and those of a y whose
+// rows do not start on 16 bytes (kVec false), turn through shared memory, two rows a warp, so that neighbouring lanes store
+// neighbours (4793 x 4304 f32 with 32 bytes a lane: 24 us).
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ qs, long long rows, long long cols,
@@ -262,7 +263,8 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
   constexpr int kLanesPerRow = kTile / 8;
   constexpr int kRowsPerPass = kQuantThreads / kLanesPerRow;
   constexpr int kPasses = kTile / kRowsPerPass;
-  __shared__ __align__(16) T turned[kVec ? 1 : kQuantThreads / 32][kVec ? 1 : 2][kVec ? 8 : kTile];
+  constexpr bool kTurn = !kVec || sizeof(T) == 4;
+  __shared__ __align__(16) T turned[kTurn ? kQuantThreads / 32 : 1][kTurn ? 2 : 1][kTurn ? kTile : 8];
   pdl_launch_dependents();
   pdl_wait();
   const long long row_tile = blockIdx.x / col_tiles;
@@ -299,7 +301,7 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
       v[2 * i] = mx_from_float<T>(f.x * scale);
       v[2 * i + 1] = mx_from_float<T>(f.y * scale);
     }
-    if constexpr (kVec) {
+    if constexpr (!kTurn) {
       T* dst = y + (r0 + r) * ld + c0 + sub * 8;
       if (r < rows_here && col_there) {
         if (sub * 8 + 8 <= cols_here) {
@@ -322,9 +324,17 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
       for (int i = 0; i < 2; ++i) {
         const int row = p * kRowsPerPass + 2 * warp + i;
         T* dst = y + (r0 + row) * ld + c0;
+        if (kVec && 4 * lane + 4 <= cols_here) {
+          if (row < rows_here) reinterpret_cast<uint4*>(dst)[lane] = reinterpret_cast<const uint4*>(turned[warp][i])[lane];
+        } else if (kVec) {
 #pragma unroll
-        for (int j = 0; j < kTile / 32; ++j)
-          if (row < rows_here && 32 * j + lane < cols_here) dst[32 * j + lane] = turned[warp][i][32 * j + lane];
+          for (int j = 0; j < 4; ++j)
+            if (row < rows_here && 4 * lane + j < cols_here) dst[4 * lane + j] = turned[warp][i][4 * lane + j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < kTile / 32; ++j)
+            if (row < rows_here && 32 * j + lane < cols_here) dst[32 * j + lane] = turned[warp][i][32 * j + lane];
+        }
       }
       __syncwarp();
     }

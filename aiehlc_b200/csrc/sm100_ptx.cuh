@@ -155,7 +155,8 @@ __device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src), "r"(c0), "r"(c1) : "memory");
 }
-// Same, but global += shared (element type and operation width come from the tensor map: int32).
+// Same, but global += shared (the element type comes from the tensor map: int32, or float, whose subnormal results may be
+// flushed to zero).
 __device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, uint32_t src, int c0, int c1) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src), "r"(c0), "r"(c1) : "memory");

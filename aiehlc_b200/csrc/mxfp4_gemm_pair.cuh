@@ -73,7 +73,8 @@ __device__ __forceinline__ void mx_unit(const MxGemmParams& p, int u, int& mb, i
 // 32 rows x 32 columns of C, one row per lane, through this warp's staging buffer and out one row at a time, neighbouring lanes
 // on neighbouring columns: for a C that allows no tile stores.  One warp per scheduler does this, so what counts is
 // the number of instructions a row takes: 26 with tests and addresses worked out per row made a 4793 x 4299 result take 62 us,
-// where tile stores take 15.  What is added to is read eight rows ahead.
+// where tile stores take 15.  Adding is one reduction per element: nothing is waited for, and as an element is added to once, the
+// result does not depend on timing.
 template <int kOut>
 __device__ __forceinline__ void store_rows(const MxGemmParams& p, uint8_t* buf, const uint32_t (&r)[32], int row0, int col0, int lane) {
   using T = std::conditional_t<kOut == MX_BF16, __nv_bfloat16, std::conditional_t<kOut == MX_F16, __half, float>>;
@@ -90,23 +91,18 @@ __device__ __forceinline__ void store_rows(const MxGemmParams& p, uint8_t* buf, 
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float*>(src + i * 128 + (((lane >> 2) ^ i) << 4));
-    T* at = c;
     if (i0 + 8 <= rows) {
-      if constexpr (kOut == MX_F32_ADD) {
-        float was[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i, at += p.ldc) was[i] = *at;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += was[i];
+      for (int i = 0; i < 8; ++i, c += p.ldc) {
+        if constexpr (kOut == MX_F32_ADD) red_add_f32(c, v[i]);
+        else *c = mx_from_float<T>(v[i]);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i, c += p.ldc) *c = mx_from_float<T>(v[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i, at += p.ldc)
+      for (int i = 0; i < 8; ++i, c += p.ldc)
         if (i0 + i < rows) {
-          if constexpr (kOut == MX_F32_ADD) v[i] += *at;
-          *at = mx_from_float<T>(v[i]);
+          if constexpr (kOut == MX_F32_ADD) red_add_f32(c, v[i]);
+          else *c = mx_from_float<T>(v[i]);
         }
     }
   }

@@ -78,8 +78,12 @@ __device__ __forceinline__ void codes_of(const Run<T, kCount>& v, int s, uint32_
 //   columns: the tile turns through shared memory; a thread takes 32 rows of two neighbouring columns, and the codes
 //            of a column's four blocks leave as 64 contiguous bytes
 // A 128 x 128 tile makes exactly one 512-byte scale tile each way, which leaves as one contiguous store.
-// Where rows do not start on 16 bytes (kVec false) the tile comes in element by element, neighbouring lanes on neighbouring
-// elements, and the rows are read back from shared memory.
+// Where rows do not start on 16 bytes (kVec false) the tile comes in by four-byte asynchronous copies and the rows are read back
+// from shared memory.
+// Elements from one staged row of the tile to the next: unaligned rows of a 16-bit type take one more word.
+template <typename T, bool kVec>
+__host__ __device__ constexpr int tile_pitch() { return sizeof(T) == 2 && !kVec ? kTile + 2 : kTile; }
+
 template <typename T, bool kVec, bool kRows, bool kCols>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 3)
 mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long long ld, uint8_t* __restrict__ q,
@@ -88,7 +92,7 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
   uint8_t* row_scales = smem;                        // 512 bytes
   uint8_t* col_scales = smem + kMxScaleTile;         // 512 bytes
   T* tile = reinterpret_cast<T*>(smem + 2 * kMxScaleTile);                          // [128][128]
-  uint8_t* turned = smem + 2 * kMxScaleTile + kTile * kTile * sizeof(T);            // codes along the columns
+  uint8_t* turned = smem + 2 * kMxScaleTile + kTile * tile_pitch<T, kVec>() * sizeof(T);   // codes along the columns
   // Elements of a row a thread takes.  Half a block where rows are quantised (4096 x 4096 bf16, rows: 6.2 us against 8.9 us with
   // a quarter); a quarter where the tile only passes through shared memory, where 32-byte strides cost bank
   // conflicts (columns: 8.7 against 9.6 us; f32 both ways, 8192 x 8192: 79 against 89 us).
@@ -97,6 +101,7 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
   constexpr int kRowsPerPass = kQuantThreads / kLanesPerRow;
   constexpr int kPasses = kTile / kRowsPerPass;
   using R = Run<T, kRun>;
+  constexpr int kPitch = tile_pitch<T, kVec>();
 
   pdl_launch_dependents();
   pdl_wait();
@@ -141,24 +146,58 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
           reinterpret_cast<uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * kRun)[i] = *reinterpret_cast<const uint4*>(&v[p].w[4 * i]);
     }
   } else {
-    const int c = tid & (kTile - 1);
-    const bool col_there = c0 + c < cols;
+    // Four bytes at a time, all of them on their way at once.  A row of a 16-bit type may start in the middle of four: its
+    // elements then start in the middle of the staged row's first word (`odd`).
+    const int cols_here = static_cast<int>(min(static_cast<long long>(kTile), cols - c0));
+    const int warp = tid >> 5, lane = tid & 31;
+    constexpr int kWords = kPitch * static_cast<int>(sizeof(T)) / 4;
+    constexpr int kWarps = kQuantThreads / 32;
+    if (rows_here == kTile && cols_here == kTile && blockIdx.x != 0) {
+      // a whole tile, and not the first (whose first word may start before the matrix): nothing to test per word
+      uintptr_t row = reinterpret_cast<uintptr_t>(x + ((r0 + warp) * ld + c0));
+      uint32_t dst = smem_u32(tile + warp * kPitch) + 4 * lane;
+#pragma unroll 4
+      for (int i = 0; i < kTile / kWarps; ++i) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(row & ~static_cast<uintptr_t>(3)) + 4 * lane;
+#pragma unroll
+        for (int w = 0; w < kTile * static_cast<int>(sizeof(T)) / 128; ++w) cp_async_4(dst + 128 * w, src + 128 * w, 4);
+        // the last element, where the row starts in the middle of a word
+        if (sizeof(T) == 2 && (row & 2) && lane == 0) cp_async_4(dst + 2 * kTile, src + 2 * kTile, 2);
+        row += kWarps * ld * sizeof(T);
+        dst += kWarps * kPitch * sizeof(T);
+      }
+    } else
 #pragma unroll 1
-    for (int r = tid / kTile; r < kTile; r += 32) {
-      T e[16];
+    for (int r = warp; r < kTile; r += kWarps) {
+      const uintptr_t row = reinterpret_cast<uintptr_t>(x + ((r0 + r) * ld + c0));
+      const int odd = static_cast<int>(row & 2) >> 1;
+      const int bytes = r < rows_here ? cols_here * static_cast<int>(sizeof(T)) + 2 * odd : 0;
+      T* dst = tile + r * kPitch;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        e[i] = col_there && r + 2 * i < rows_here ? x[(r0 + r + 2 * i) * ld + c0 + c] : mx_from_float<T>(0.0f);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) tile[(r + 2 * i) * kTile + c] = e[i];
+      for (int w = lane; w < kWords; w += 32) {
+        if (4 * w >= bytes) reinterpret_cast<uint32_t*>(dst)[w] = 0;
+        else if (odd && w == 0 && r0 + r == 0 && c0 == 0) dst[1] = x[0];   // nothing before the matrix is read
+        else cp_async_4(smem_u32(dst) + 4 * w, reinterpret_cast<const uint8_t*>(row - 2 * odd) + 4 * w, min(4, bytes - 4 * w));
+      }
     }
+    cp_async_wait_all();
+    __syncthreads();
     if constexpr (kRows) {
-      __syncthreads();
 #pragma unroll
-      for (int p = 0; p < kPasses; ++p)
+      for (int p = 0; p < kPasses; ++p) {
+        const T* src = tile + (p * kRowsPerPass + line) * kPitch + sub * kRun;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < R::kPieces; ++i)
-          *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = reinterpret_cast<const uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * kRun)[i];
+          for (int i = 0; i < R::kPieces; ++i) *reinterpret_cast<uint4*>(&v[p].w[4 * i]) = reinterpret_cast<const uint4*>(src)[i];
+        } else {
+          const bool odd = reinterpret_cast<uintptr_t>(x + ((r0 + p * kRowsPerPass + line) * ld + c0)) & 2;
+          uint32_t w[R::kWords + 1];
+#pragma unroll
+          for (int i = 0; i <= R::kWords; ++i) w[i] = reinterpret_cast<const uint32_t*>(src)[i];
+#pragma unroll
+          for (int i = 0; i < R::kWords; ++i) v[p].w[i] = odd ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+        }
+      }
     }
   }
   if constexpr (kRows) {
@@ -192,14 +231,14 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
     constexpr int kTurnedPitch = 80;                 // 64 bytes of codes per column; the pad spreads the banks
     const long long row_blocks = mx_blocks(rows);
     const int pair = tid & 63, rb = tid >> 6;        // columns 2 pair, 2 pair + 1; rows 32 rb ...
-    const T* src = tile + rb * kMxBlock * kTile + 2 * pair;
+    const T* src = tile + rb * kMxBlock * kPitch + 2 * pair;
     uint32_t m0, m1;
     float f0[kMxBlock], f1[kMxBlock];
     if constexpr (sizeof(T) == 4) {
       m0 = m1 = 0;
 #pragma unroll
       for (int i = 0; i < kMxBlock; ++i) {
-        const float2 f = *reinterpret_cast<const float2*>(src + i * kTile);
+        const float2 f = *reinterpret_cast<const float2*>(src + i * kPitch);
         f0[i] = f.x;
         f1[i] = f.y;
         m0 = max(m0, __float_as_uint(f.x) & 0x7FFFFFFFu);
@@ -209,7 +248,11 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < kMxBlock; ++i) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(src + i * kTile);
+        uint32_t w = *reinterpret_cast<const uint32_t*>(src + i * kPitch);
+        if constexpr (!kVec) {
+          const uint32_t next = *reinterpret_cast<const uint32_t*>(src + i * kPitch + 2);
+          if (reinterpret_cast<uintptr_t>(x + ((r0 + rb * kMxBlock + i) * ld + c0)) & 2) w = __funnelshift_r(w, next, 16);
+        }
         const float2 f = split2<T>(w);
         f0[i] = f.x;
         f1[i] = f.y;
@@ -357,7 +400,7 @@ cudaLaunchConfig_t tile_grid(const aiehlc_ctx* ctx, unsigned tiles, int smem, cu
 template <typename T, bool kVec, bool kRows, bool kCols>
 int quantize_as(aiehlc_ctx* ctx, const MxQuantizeCall& c, cudaStream_t st) {
   auto kern = mx_quantize_kernel<T, kVec, kRows, kCols>;
-  const int smem = 2 * kMxScaleTile + (kCols || !kVec ? kTile * kTile * static_cast<int>(sizeof(T)) : 0) + (kCols ? kTile * 80 : 0);
+  const int smem = 2 * kMxScaleTile + (kCols || !kVec ? kTile * tile_pitch<T, kVec>() * static_cast<int>(sizeof(T)) : 0) + (kCols ? kTile * 80 : 0);
   KernelSetup& ks = ctx->kernel_setup[reinterpret_cast<const void*>(kern)];
   if (int rc = ensure_dynamic_smem(ctx->device, reinterpret_cast<const void*>(kern), smem, &ks.smem_attr)) return rc;
   const int col_tiles = static_cast<int>((c.cols + kTile - 1) / kTile);

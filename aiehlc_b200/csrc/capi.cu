@@ -558,7 +558,9 @@ static int check_mx_product(const void* A, const void* As, const void* B, const 
 }
 static int check_mx_sizes(int M, int N, int K, const char* what) {
   if (M < 0 || N < 0 || K < 0) return fail(AIEHLC_ERR_INVALID, std::string(what) + ": negative size");
-  if (M > 1 << 30 || N > 1 << 30 || K > 1 << 30) return fail(AIEHLC_ERR_UNSUPPORTED, std::string(what) + ": M, N, K up to 2^30");
+  if (M > 1 << 30 || N > 1 << 30) return fail(AIEHLC_ERR_UNSUPPORTED, std::string(what) + ": M and N up to 2^30");
+  // a tile's main loop stays well inside the kernels' one-second limit on waits
+  if (K > 1 << 26) return fail(AIEHLC_ERR_UNSUPPORTED, std::string(what) + ": K up to 2^26");
   // one CTA (or pair) per output tile, at most eight times as many with K split
   if ((M / 128 + 1LL) * (N / 128 + 1LL) > 1LL << 28) return fail(AIEHLC_ERR_UNSUPPORTED, std::string(what) + ": too many output tiles");
   return AIEHLC_OK;

@@ -152,7 +152,7 @@ int aiehlc_dequantize_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* q, const uint8_t
 /* C[i][j] = sum_k A[i][k] * B[j][k] of quantised A [M][K] and B [N][K], sums in 32-bit floating point, C of `type` with row
  * pitch `ldc` elements (>= N), rounded once.  accumulate != 0 (type AIEHLC_TYPE_F32 only): C += A.B^T, one addition per
  * element (sums below 2^-126 in magnitude may become zero).  Results do not depend on timing.
- * M, N, K up to 2^30. */
+ * M and N up to 2^30, K up to 2^26; C may not overlap the operands. */
 int aiehlc_gemm_mxfp4_dev(aiehlc_ctx* ctx, const uint8_t* A, const uint8_t* A_scales, const uint8_t* B,
                           const uint8_t* B_scales, void* C, int type, int M, int N, int K, long long ldc, int accumulate,
                           void* stream);

@@ -360,6 +360,95 @@ def test_a_wait_that_runs_out_is_reported_and_the_context_survives(M, N, K):
         c.close()
 
 
+def test_one_matrix_as_both_operands(ctx):
+    (A, a) = _whole(300, 500, 1)
+    assert np.array_equal(ctx.gemm_mxfp4(A, A, torch.float32).double().cpu().numpy(), a @ a.T) and ctx.sync() == 0
+
+
+def test_among_other_kernels_without_a_pause(ctx):
+    """Launches that start while the one before drains (and hold TMEM then): int8 and 4-bit products of both forms,
+    quantisation and values in one stream, each reading what the call before has written."""
+    (A, a), (B, b) = _whole(300, 512, 1), _whole(512, 512, 2)
+    i8 = torch.randint(-8, 8, (256, 256), dtype=torch.int8, device=DEV)
+    want8 = (i8.float() @ i8.float().t()).int()
+    outs, ref = [], None
+    for _ in range(30):
+        c = ctx.gemm_mxfp4(A, B, torch.float32)
+        r, t = ctx.quantize_mxfp4(c, "both")
+        d = ctx.gemm_mxfp4(r, B, torch.float32)
+        e = ctx.gemm_i8_i32(i8, i8)
+        q = ctx.gemm_mxfp4_mxfp4(MxFp4(r.codes[:16], r.scales[:2048], 16, 512), B)
+        outs.append((c, d, e, ctx.dequantize_mxfp4(q, torch.float32), ctx.dequantize_mxfp4(t, torch.float32)))
+    assert ctx.sync() == 0
+    m = X.rounded(a @ b.T)
+    assert np.array_equal(outs[0][0].double().cpu().numpy(), a @ b.T)
+    assert (np.abs(outs[0][1].double().cpu().numpy() - m @ b.T) <= _bound(m, b, 512, "f32")).all()
+    assert np.array_equal(outs[0][3].double().cpu().numpy(), X.rounded(outs[0][1][:16].double().cpu().numpy()))
+    assert np.array_equal(outs[0][4].double().cpu().numpy(), X.rounded((a @ b.T).T))
+    for c, d, e, f, g in outs:
+        assert torch.equal(e, want8)
+        assert all(torch.equal(x, y) for x, y in zip((c, d, f, g), (outs[0][i] for i in (0, 1, 3, 4))))
+
+
+def test_two_streams_at_once(ctx):
+    sets = [_whole(m, 1030, m) + _whole(700, 1030, m + 1) for m in (5, 300, 40, 1000)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[] for _ in sets]
+    for _ in range(10):
+        for s, (A, _, B, _), g in zip(streams, sets, got):
+            with torch.cuda.stream(s):
+                g.append(ctx.gemm_mxfp4(A, B, torch.float32))
+    torch.cuda.synchronize()
+    for (_, a, _, b), g in zip(sets, got):
+        assert all(np.array_equal(c.double().cpu().numpy(), a @ b.T) for c in g)
+    assert ctx.sync() == 0
+
+
+@pytest.mark.parametrize("sms", [1, 2, 7, 64])
+def test_a_limit_on_the_sms(sms):
+    c = Context(0)
+    try:
+        c.set_cta_limit(sms)
+        for M, N, K in ((3, 700, 1030), (100, 300, 2048), (600, 900, 520)):
+            (A, a), (B, b) = _whole(M, K, 1), _whole(N, K, 2)
+            assert np.array_equal(c.gemm_mxfp4(A, B, torch.float32).double().cpu().numpy(), a @ b.T)
+            _same(c.gemm_mxfp4_mxfp4(A, B, out=_poisoned(M, N)), a @ b.T)
+        assert c.sync() == 0
+    finally:
+        c.close()
+
+
+def test_offsets_past_32_bits(ctx):
+    """More than 2^32 elements (2^31 bytes of codes): the last rows are where 32-bit offsets would go wrong."""
+    rows, cols = 131100, 33000
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(1))
+    r, t = ctx.quantize_mxfp4(x, "both")
+    at = torch.tensor([0, 1, 65077, 130175, 131098, 131099], device=DEV)
+    want = X.rounded(x[at].double().cpu().numpy())
+    v = ctx.dequantize_mxfp4(r)
+    assert np.array_equal(v[at].double().cpu().numpy(), want)
+    del v
+    cols_at = torch.tensor([0, 31, 16001, 32998, 32999], device=DEV)
+    want_t = X.rounded(x[:, cols_at].double().cpu().numpy().T)
+    del x
+    v = ctx.dequantize_mxfp4(t)
+    assert np.array_equal(v[cols_at].double().cpu().numpy(), want_t)
+    del v, t
+    (B, b) = _quantized(8, cols, 3)
+    c = ctx.gemm_mxfp4(B, r, torch.float32)                                   # long rows, many of them
+    assert (np.abs(c[:, at].double().cpu().numpy() - b @ want.T) <= _bound(b, want, cols, "f32")).all()
+    del c, r
+    (A, a), (B, b) = _whole(rows, 64, 5), _whole(cols, 64, 6)
+    c = ctx.gemm_mxfp4(A, B)                                                  # a result of more than 2^32 elements
+    ref = torch.from_numpy(a[at.cpu().numpy()] @ b.T).to(torch.bfloat16)
+    assert torch.equal(c[at].cpu(), ref)
+    del c
+    q = ctx.gemm_mxfp4_mxfp4(A, B)
+    v = ctx.dequantize_mxfp4(q)
+    assert np.array_equal(v[at].double().cpu().numpy(), X.rounded(a[at.cpu().numpy()] @ b.T)) and ctx.sync() == 0
+
+
 # ---------------------------------------------------------------- refusals of the Python face
 def test_refusals(ctx):
     x = torch.randn(40, 64, device=DEV)

@@ -77,6 +77,8 @@ __device__ __forceinline__ void codes_of(const Run<T, kCount>& v, int s, uint32_
 //   rows   : the lanes that hold a block agree on its maximum with shuffles; each writes the codes of its elements
 //   columns: the tile turns through shared memory; a thread takes 32 rows of two neighbouring columns, and the codes
 //            of a column's four blocks leave as 64 contiguous bytes
+// Four CTAs on an SM keep the loads of one under the arithmetic of others (16384 x 16384 bf16, rows: 96 us and 7.1 TB/s, of which
+// part comes from L2, against 105 us with three; both ways 148 against 160 us).
 // A 128 x 128 tile makes exactly one 512-byte scale tile each way, which leaves as one contiguous store.
 // Where rows do not start on 16 bytes (kVec false) the tile comes in by four-byte asynchronous copies and the rows are read back
 // from shared memory.
@@ -85,7 +87,7 @@ template <typename T, bool kVec>
 __host__ __device__ constexpr int tile_pitch() { return sizeof(T) == 2 && !kVec ? kTile + 2 : kTile; }
 
 template <typename T, bool kVec, bool kRows, bool kCols>
-__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 3)
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4)
 mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long long ld, uint8_t* __restrict__ q,
                    uint8_t* __restrict__ qs, uint8_t* __restrict__ t, uint8_t* __restrict__ ts, int col_tiles) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -94,9 +96,12 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
   T* tile = reinterpret_cast<T*>(smem + 2 * kMxScaleTile);                          // [128][128]
   uint8_t* turned = smem + 2 * kMxScaleTile + kTile * tile_pitch<T, kVec>() * sizeof(T);   // codes along the columns
   // Elements of a row a thread takes.  Half a block where rows are quantised (4096 x 4096 bf16, rows: 6.2 us against 8.9 us with
-  // a quarter); a quarter where the tile only passes through shared memory, where 32-byte strides cost bank
-  // conflicts (columns: 8.7 against 9.6 us; f32 both ways, 8192 x 8192: 79 against 89 us).
+  // a quarter); a quarter of f32 tiles that pass through shared memory, where 64-byte strides cost bank conflicts
+  // (both ways, 8192 x 8192: 79 against 89 us), and of tiles that only pass through.
   constexpr int kRun = kCols && (!kRows || sizeof(T) == 4) ? 8 : 16;
+  // Two 16-byte pieces a thread: in the second half of a row neighbouring pieces change places, so that eight threads that
+  // store their first (or second) pieces together meet all banks once.
+  constexpr bool kSwap = kVec && kCols && kRun == 16 && sizeof(T) == 2;
   constexpr int kLanesPerRow = kTile / kRun;
   constexpr int kRowsPerPass = kQuantThreads / kLanesPerRow;
   constexpr int kPasses = kTile / kRowsPerPass;
@@ -143,7 +148,8 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
       for (int p = 0; p < kPasses; ++p)
 #pragma unroll
         for (int i = 0; i < R::kPieces; ++i)
-          reinterpret_cast<uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * kRun)[i] = *reinterpret_cast<const uint4*>(&v[p].w[4 * i]);
+          reinterpret_cast<uint4*>(tile + (p * kRowsPerPass + line) * kTile + sub * kRun)[kSwap ? i ^ (sub >> 2) : i] =
+              *reinterpret_cast<const uint4*>(&v[p].w[4 * i]);
     }
   } else {
     // Four bytes at a time, all of them on their way at once.  A row of a 16-bit type may start in the middle of four: its
@@ -231,53 +237,49 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
     constexpr int kTurnedPitch = 80;                 // 64 bytes of codes per column; the pad spreads the banks
     const long long row_blocks = mx_blocks(rows);
     const int pair = tid & 63, rb = tid >> 6;        // columns 2 pair, 2 pair + 1; rows 32 rb ...
-    const T* src = tile + rb * kMxBlock * kPitch + 2 * pair;
-    uint32_t m0, m1;
-    float f0[kMxBlock], f1[kMxBlock];
-    if constexpr (sizeof(T) == 4) {
-      m0 = m1 = 0;
-#pragma unroll
-      for (int i = 0; i < kMxBlock; ++i) {
-        const float2 f = *reinterpret_cast<const float2*>(src + i * kPitch);
-        f0[i] = f.x;
-        f1[i] = f.y;
-        m0 = max(m0, __float_as_uint(f.x) & 0x7FFFFFFFu);
-        m1 = max(m1, __float_as_uint(f.y) & 0x7FFFFFFFu);
-      }
-    } else {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < kMxBlock; ++i) {
-        uint32_t w = *reinterpret_cast<const uint32_t*>(src + i * kPitch);
-        if constexpr (!kVec) {
-          const uint32_t next = *reinterpret_cast<const uint32_t*>(src + i * kPitch + 2);
-          if (reinterpret_cast<uintptr_t>(x + ((r0 + rb * kMxBlock + i) * ld + c0)) & 2) w = __funnelshift_r(w, next, 16);
-        }
-        const float2 f = split2<T>(w);
-        f0[i] = f.x;
-        f1[i] = f.y;
-        m = max_abs2<T>(m, w);
-      }
-      const float2 f = split2<T>(m);
-      m0 = __float_as_uint(f.x) & 0x7FFFFFFFu;
-      m1 = __float_as_uint(f.y) & 0x7FFFFFFFu;
-    }
+    const T* src = tile + rb * kMxBlock * kPitch + (kSwap ? (pair * 2) ^ ((pair >> 5) << 3) : 2 * pair);
     const bool block_there = r0 / kMxBlock + rb < row_blocks;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    // codes and scale of column 2 pair + h
+    const auto column = [&](int h, uint32_t most, const auto& value) {
       const int c = 2 * pair + h;
-      const int s = mx_scale_of(h ? m1 : m0);
+      const int s = mx_scale_of(most & 0x7FFFFFFFu);
       const float inv = mx_inverse(s);
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float g[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = (h ? f1[8 * j + i] : f0[8 * j + i]) * inv;
+        for (int i = 0; i < 8; ++i) g[i] = value(8 * j + i) * inv;
         w[j] = s == kMxNan ? 0u : mx_codes8(g);
       }
-      *reinterpret_cast<uint4*>(turned + c * kTurnedPitch + rb * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(turned + c * kTurnedPitch + (rb ^ ((c >> 3) & 1)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
       col_scales[mx_scale_word(c) + rb] = block_there && c0 + c < cols ? static_cast<uint8_t>(s) : 0;
+    };
+    if constexpr (sizeof(T) == 4) {
+      float2 f[kMxBlock];
+      uint32_t m0 = 0, m1 = 0;
+#pragma unroll
+      for (int i = 0; i < kMxBlock; ++i) {
+        f[i] = *reinterpret_cast<const float2*>(src + i * kPitch);
+        m0 = max(m0, __float_as_uint(f[i].x) & 0x7FFFFFFFu);
+        m1 = max(m1, __float_as_uint(f[i].y) & 0x7FFFFFFFu);
+      }
+      column(0, m0, [&](int i) { return f[i].x; });
+      column(1, m1, [&](int i) { return f[i].y; });
+    } else {
+      uint32_t w[kMxBlock], m = 0;
+#pragma unroll
+      for (int i = 0; i < kMxBlock; ++i) {
+        w[i] = *reinterpret_cast<const uint32_t*>(src + i * kPitch);
+        if constexpr (!kVec) {
+          const uint32_t next = *reinterpret_cast<const uint32_t*>(src + i * kPitch + 2);
+          if (reinterpret_cast<uintptr_t>(x + ((r0 + rb * kMxBlock + i) * ld + c0)) & 2) w[i] = __funnelshift_r(w[i], next, 16);
+        }
+        m = max_abs2<T>(m, w[i]);
+      }
+      const float2 f = split2<T>(m);
+      column(0, __float_as_uint(f.x), [&](int i) { return split2<T>(w[i]).x; });
+      column(1, __float_as_uint(f.y), [&](int i) { return split2<T>(w[i]).y; });
     }
     __syncthreads();
     // four threads per column: its four blocks' codes are 64 contiguous bytes
@@ -287,7 +289,7 @@ mx_quantize_kernel(const T* __restrict__ x, long long rows, long long cols, long
       const long long block = r0 / kMxBlock + b;
       if (c0 + c < cols && block < row_blocks)
         *reinterpret_cast<uint4*>(t + ((c0 + c) * row_blocks + block) * 16) =
-            *reinterpret_cast<const uint4*>(turned + c * kTurnedPitch + b * 16);
+            *reinterpret_cast<const uint4*>(turned + c * kTurnedPitch + (b ^ ((c >> 3) & 1)) * 16);
     }
     if (tid < kMxScaleTile / 16)
       reinterpret_cast<uint4*>(ts + (static_cast<long long>(col_tile) * mx_words(rows) + row_tile) * kMxScaleTile)[tid] =

@@ -60,6 +60,18 @@ def plan_tile_order(M: int, N: int, K: int, kind: str = "int8", num_shards: int 
     return rb[:got], cb[:got], int(slots.value)
 
 
+_torch_module = None
+
+
+def _torch():
+    """torch, imported when it is first needed (the host entry points do without it)."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
+
+
 class MxFp4:
     """A microscaled 4-bit matrix [rows][cols]: 32 consecutive elements of a row share a power of two (the format and the
     layout of the two arrays: aiehlc_b200.h).
@@ -73,16 +85,19 @@ class MxFp4:
     __slots__ = ("rows", "cols", "device_index", "_codes", "_scales", "_whole", "_at")
 
     def __init__(self, codes, scales, rows: int, cols: int):
-        import torch
+        torch = _torch()
         if rows < 0 or cols < 0:
             raise ValueError("MxFp4: negative size")
-        index = codes.get_device() if isinstance(codes, torch.Tensor) else -1
-        for t, n, size in ((codes, "codes", rows * ((cols + 31) // 32 * 16)),
-                           (scales, "scales", (rows + 127) // 128 * ((cols + 127) // 128) * 512)):
-            if not isinstance(t, torch.Tensor) or t.dtype is not torch.uint8 or t.get_device() != index or index < 0:
-                raise TypeError(f"MxFp4: {n}: expected a uint8 CUDA tensor, codes and scales on one device")
-            if t.numel() != size or not t.is_contiguous():
-                raise ValueError(f"MxFp4: {n}: expected {size} contiguous bytes for {rows} x {cols}")
+        if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+            raise TypeError("MxFp4: expected uint8 CUDA tensors for codes and scales")
+        index = codes.get_device()
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or index < 0 or scales.get_device() != index:
+            raise TypeError("MxFp4: expected uint8 CUDA tensors, codes and scales on one device")
+        if codes.numel() != rows * ((cols + 31) // 32 * 16) or not codes.is_contiguous():
+            raise ValueError(f"MxFp4: codes: expected {rows * ((cols + 31) // 32 * 16)} contiguous bytes for {rows} x {cols}")
+        if scales.numel() != (rows + 127) // 128 * ((cols + 127) // 128) * 512 or not scales.is_contiguous():
+            raise ValueError(f"MxFp4: scales: expected {(rows + 127) // 128 * ((cols + 127) // 128) * 512} contiguous bytes for "
+                             f"{rows} x {cols}")
         self.rows, self.cols, self.device_index = rows, cols, index
         self._codes, self._scales, self._whole = codes, scales, None
         self._at = (codes.data_ptr(), scales.data_ptr())

@@ -15,7 +15,7 @@ namespace {
 
 enum : int { MX_F32 = 0, MX_F32_ADD = 1, MX_BF16 = 2, MX_F16 = 3, MX_MX = 4 };
 
-constexpr int kStepK = 256;                    // elements of K per stage: one 128-byte swizzle span of codes
+constexpr int kStepK = 256;                    // elements of K per step: one 128-byte swizzle span of codes
 constexpr int kStepScales = 2 * kMxScaleTile;  // two scale tiles of 4 blocks each
 constexpr int kMmaK = 64;                      // elements of K per tcgen05.mma
 constexpr int kKPer = 2;                       // steps per pipeline stage

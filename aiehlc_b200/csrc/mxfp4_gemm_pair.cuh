@@ -1,19 +1,18 @@
 // Products of microscaled 4-bit matrices by CTA pairs (tcgen05 cta_group::2): two CTAs on neighbouring SMs share one
 // 256 x kBN tile of C, persistent over the tiles.  Included by mxfp4_gemm.cu.
 //
-//   warp 0 (both CTAs)  fetches this CTA's 128 rows of A and its half of B's rows (credited to the leader's "full"
-//                       barrier), the scales of its A rows and those of all of the tile's B rows (each CTA multiplies with
-//                       all of B; credited to its own "scales full" barrier)
-//   warp 1 (leader)     issues the products, M = 256, K = 64 each
+//   warp 0 (both CTAs)  fetches this CTA's 128 rows of A, its half of B's rows, the scales of its A rows and the scales of all
+//                       of the tile's B rows (each CTA multiplies with all of B); everything is credited to the
+//                       leader's "full" barrier
+//   warp 1 (leader)     copies the scales to both CTAs' TMEM and issues the products, M = 256, K = 64 each
 //   warps 2-5           drain this CTA's 128 accumulator rows through the output stage
-//   warps 6-9           move the scales from shared memory to this CTA's TMEM, one lane quarter each
 //
-// Why warps and not tcgen05.cp: the copies run in the tensor cores' own queue, between the products, not beside them.  Measured
-// on 512 x 9472 x 65536 (one tile per pair): 166 cycles per product without copies, 240 with six 512-byte copies per four
-// products (about 30 cycles a copy and 64 each time the queue turns from products to copies), 313 with the
-// commits that tell when a set of scales may be overwritten.
+// What the products take is set by the issuing warp as much as by the tensor cores (256 x 256 x 64: 128 cycles).  Under
+// `if (lane == 0)` a product took 155 cycles and the scale copies 75 more; with the whole warp walking the loop and one elected
+// lane issuing, 129 and nothing (512 x 9472 x 65536, operands not loaded; 160 with them).  Four warps that wrote
+// the scales with tcgen05.st instead of the copies: 199 against 193 us on 8192^3, 13.5 against 12.8 on 4096 x 4096 x 1024.
 //
-// TMEM (512 columns per CTA): two accumulators of kBN columns and kSets sets of scales, one per stage in flight: for each
+// TMEM (512 columns per CTA): two accumulators of kBN columns and two sets of scales, one per stage in flight: for each
 // 128 elements of K, 4 columns of A's scales and kBN / 32 of B's.  With kBN = 256 the accumulators share 96 columns, which
 // makes the room: accumulator 0 takes columns 0-255, accumulator 1 columns 160-415.  The output stage reads the
 // half of a tile that holds the shared columns first and hands them back at once, so that the next tile's products
@@ -24,7 +23,7 @@ namespace aiehlc {
 
 namespace {
 
-constexpr int kMxPairThreads = 320;
+constexpr int kMxPairThreads = 192;
 // A stage holds kKPer steps of K: a commit costs the tensor cores' queue about 50 cycles (measured: 166 cycles per product
 // with one commit per eight products, 179 with one more per four), so a stage is as long as shared memory allows.
 template <int kBN>
@@ -46,7 +45,7 @@ struct MxPairShape {
   static constexpr int kAcc1 = kBN == 256 ? 160 : kBN;         // first column of accumulator 1
   static constexpr int kWordCols = 4 + 4 * kBTiles;            // columns of scales per 128 elements of K
   static constexpr int kSetCols = 2 * kKPer * kWordCols;
-  static constexpr int kSets = 4 / kKPer;
+  static constexpr int kSets = 2;
   static constexpr int kScaleCol = kAcc1 + kBN;
   static constexpr int kTmemCols = 512;
   static_assert(kStageBytes % 1024 == 0 && kScaleCol + kSets * kSetCols <= kTmemCols && kSets <= kStages, "layout");
@@ -120,9 +119,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   uint8_t* staging = smem + kStages * S::kStageBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + S::kStagingBytes);  // used in the leader
   uint64_t* empty_bar = full_bar + kStages;           // one set per CTA
-  uint64_t* scales_full_bar = empty_bar + kStages;    // one set per CTA
-  uint64_t* scales_set_bar = scales_full_bar + kStages;  // used in the leader: a set of scales is in TMEM
-  uint64_t* tmem_full_bar = scales_set_bar + S::kSets;   // one set per CTA
+  uint64_t* tmem_full_bar = empty_bar + kStages;      // one set per CTA
   uint64_t* tmem_free_bar = tmem_full_bar + 2;        // used in the leader: one per accumulator, or one for what they share
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_free_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
@@ -138,9 +135,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
-      mbar_init(smem_u32(&scales_full_bar[s]), 1);
     }
-    for (int a = 0; a < S::kSets; ++a) mbar_init(smem_u32(&scales_set_bar[a]), 8);  // the scale warps of the two CTAs
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&tmem_full_bar[a]), 1);
       mbar_init(smem_u32(&tmem_free_bar[a]), 8);      // every output warp of the two CTAs
@@ -183,7 +178,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           ok = mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status, ST_TIMEOUT_EMPTY);
           if (!ok) break;
           if (p.debug != 3) {
-            if (leader) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * (S::kABytes + kKPer * 128 * b_rows));
+            if (leader) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * (S::kABytes + kKPer * 128 * b_rows + S::kAScales + S::kBScales));
             const uint32_t bar = mapa_u32(smem_u32(&full_bar[stage]), 0);
             const uint32_t sa = smem_u32(smem + stage * S::kStageBytes);
             const uint32_t sb = sa + S::kABytes;
@@ -200,10 +195,8 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
                 tma_load_2d_pair(sb + kk * 128 * b_rows, map_b, bar, (k + kk) * 128, row_b);
               }
             }
-            const uint32_t scales_bar = smem_u32(&scales_full_bar[stage]);
-            mbar_expect_tx(scales_bar, S::kAScales + S::kBScales);
-            tma_load_2d(ss, &tmap_as, scales_bar, k * (kStepScales / 8), mb * 2 + rank);
-            tma_load_2d(ss + S::kAScales, &tmap_bs, scales_bar, k * (kStepScales / 8), scales_b);
+            tma_load_2d_pair(ss, &tmap_as, bar, k * (kStepScales / 8), mb * 2 + rank);
+            tma_load_2d_pair(ss + S::kAScales, &tmap_bs, bar, k * (kStepScales / 8), scales_b);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
@@ -216,7 +209,9 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       int stage = 0;
       uint32_t phase = 0;
       int set = 0;
-      uint32_t set_phase = 0;
+      int old_stage = 0;                              // whose products have read the set before it is written again
+      uint32_t old_phase = 0;
+      bool reuse = false;
       int it = 0;
       bool ok = true;
       for (int t = pair_id; ok && t < num_units; t += num_pairs, ++it) {
@@ -232,8 +227,12 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         const uint32_t idesc = halved ? make_idesc_mxf4(256, kBN / 2, 0) : make_idesc_mxf4(256, kBN, 0);
         const uint32_t b_block = S::kBBlock >> (halved ? 5 : 4);   // descriptor units from one step of K to the next
         for (int k = 0; k < p.k_steps; k += kKPer) {
-          ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL) &&
-               mbar_wait(smem_u32(&scales_set_bar[set]), set_phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+          ok = mbar_wait(smem_u32(&full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL);
+          if (reuse) {
+            // the stage before keeps the tensor cores busy meanwhile
+            ok = ok && mbar_wait(smem_u32(&empty_bar[old_stage]), old_phase, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY);
+            if (++old_stage == kStages) { old_stage = 0; old_phase ^= 1; }
+          }
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -249,6 +248,14 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
                            bdesc + ((i / kPerStep) * b_block + 2 * (i % kPerStep)), idesc | make_idesc_mxf4_scale(2 * (i & 1)),
                            t_scales + (i >> 1) * S::kWordCols, t_scales + (i >> 1) * S::kWordCols + 4, accumulate);
             };
+            const uint64_t sdesc = make_scale_desc(sa + S::kABytes + S::kBBytes);
+#pragma unroll
+            for (int w = 0; w < 2 * kKPer; ++w) {
+              tmem_copy_scales<2>(t_scales + w * S::kWordCols, sdesc + ((w * kMxScaleTile) >> 4));
+#pragma unroll
+              for (int b = 0; b < S::kBTiles; ++b)
+                tmem_copy_scales<2>(t_scales + w * S::kWordCols + 4 + 4 * b, sdesc + ((S::kAScales + (b * 2 * kKPer + w) * kMxScaleTile) >> 4));
+            }
             product(0, k > 0);
             if (mmas == kKPer * kPerStep) {   // straight through: a test per product costs the issuing thread 20 to 40 cycles
 #pragma unroll
@@ -261,51 +268,11 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             umma_commit_pair_mask(smem_u32(&empty_bar[stage]), 3);
           }
           __syncwarp();
-          if (++set == S::kSets) { set = 0; set_phase ^= 1; }
+          if (++set == S::kSets) { set = 0; reuse = true; }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
         if (ok && elect_one()) umma_commit_pair_mask(smem_u32(&tmem_full_bar[it & 1]), 3);
         __syncwarp();
-      }
-    }
-  } else if (warp >= 6) {
-    // A stage's scales: the 16-byte line of this lane in every scale tile is four columns of TMEM.  A set of columns is free
-    // once the products of the stage kSets before are done, which is what that stage's "empty" barrier says.
-    const int quad = warp & 3;
-    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + S::kScaleCol;
-    int stage = 0, set = 0, old_stage = 0;
-    uint32_t phase = 0, old_phase = 0;
-    long long used = 0;
-    bool ok = true;
-    for (int t = pair_id; ok && t < num_units; t += num_pairs) {
-      for (int k = 0; k < p.k_steps; k += kKPer) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&scales_full_bar[stage]), phase, abort_flag, p.status, ST_TIMEOUT_FULL));
-        if (!ok) break;
-        const uint8_t* ss = smem + stage * S::kStageBytes + S::kABytes + S::kBBytes;
-        alignas(16) uint32_t r[S::kSetCols];
-#pragma unroll
-        for (int w = 0; w < 2 * kKPer; ++w) {
-          *reinterpret_cast<uint4*>(&r[w * S::kWordCols]) = *reinterpret_cast<const uint4*>(ss + w * kMxScaleTile + lane * 16);
-#pragma unroll
-          for (int b = 0; b < S::kBTiles; ++b)
-            *reinterpret_cast<uint4*>(&r[w * S::kWordCols + 4 + 4 * b]) =
-                *reinterpret_cast<const uint4*>(ss + S::kAScales + (b * 2 * kKPer + w) * kMxScaleTile + lane * 16);
-        }
-        if (used >= S::kSets) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty_bar[old_stage]), old_phase, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY));
-          if (!ok) break;
-          tc_fence_after();
-          if (++old_stage == kStages) { old_stage = 0; old_phase ^= 1; }
-        }
-        ++used;
-#pragma unroll
-        for (int c = 0; c < S::kSetCols; c += 8) tmem_st_32x32b_x8(t_lane + set * S::kSetCols + c, &r[c]);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_remote(smem_u32(&scales_set_bar[set]), 0);
-        if (++set == S::kSets) set = 0;
-        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
   } else {

@@ -271,15 +271,6 @@ __device__ __forceinline__ void tmem_ld_wait() {
 }
 
 
-// The other way: thread t of the warp writes lane (base+t), r[j] to column j.
-__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
-               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
 // ------------------------------------------------------------------ cross-CTA flags in global memory
 __device__ __forceinline__ int ld_acquire_gpu(const int* p) {
   int v;

@@ -319,12 +319,14 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int n = n0 + c + 32 * h;
+            if (n + 32 > p.N) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (n + j >= p.N) r[h][j] = 0;
+            }
             uint32_t most = 0;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (n + j >= p.N) r[h][j] = 0;
-              most = max(most, r[h][j] & 0x7FFFFFFFu);
-            }
+            for (int j = 0; j < 32; ++j) most = max(most, r[h][j] & 0x7FFFFFFFu);
             const int s = mx_scale_of(most);
             const float inv = mx_inverse(s);
             uint32_t w[4];

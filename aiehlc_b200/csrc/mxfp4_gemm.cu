@@ -67,7 +67,8 @@ struct NarrowShape {
   static_assert(kTN + kScaleCols <= kTmemCols, "TMEM");
 };
 
-// Stores four consecutive results of a row; `n` is the first one's column.
+// Stores four consecutive results of a row; `n` is the first one's column.  Adding is a reduction, as in the other form: nothing
+// is waited for, and each element is added to once.
 template <int kOut>
 __device__ __forceinline__ void store4(const MxGemmParams& p, int m, int n, const float4& v) {
   const long long at = static_cast<long long>(m) * p.ldc + n;
@@ -75,16 +76,15 @@ __device__ __forceinline__ void store4(const MxGemmParams& p, int m, int n, cons
   if constexpr (kOut == MX_F32 || kOut == MX_F32_ADD) {
     float* c = static_cast<float*>(p.C) + at;
     if (p.vec_ok && n + 4 <= p.N) {
-      float4 o = v;
-      if constexpr (kOut == MX_F32_ADD) {
-        const float4 was = *reinterpret_cast<const float4*>(c);
-        o.x += was.x; o.y += was.y; o.z += was.z; o.w += was.w;
-      }
-      *reinterpret_cast<float4*>(c) = o;
+      if constexpr (kOut == MX_F32_ADD) red_add_f32x4(c, v);
+      else *reinterpret_cast<float4*>(c) = v;
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (n + i < p.N) c[i] = kOut == MX_F32_ADD ? c[i] + f[i] : f[i];
+        if (n + i < p.N) {
+          if constexpr (kOut == MX_F32_ADD) red_add_f32(c + i, f[i]);
+          else c[i] = f[i];
+        }
     }
   } else {
     uint16_t h[4];

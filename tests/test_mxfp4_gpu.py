@@ -155,7 +155,8 @@ def test_product(ctx, M, N, K, kind):
     assert torch.equal(out[:, :N], got) and bool((out[:, N:] == 5).all()) and ctx.sync() == 0
 
 
-@pytest.mark.parametrize("M,N,K", [(3, 70, 100), (65, 128, 300), (300, 520, 1030)])
+@pytest.mark.parametrize("M,N,K", [(3, 70, 100), (3, 72, 100), (65, 128, 300), (67, 1001, 4103), (300, 520, 1030), (300, 519, 1030),
+                                   (2500, 2000, 300)])
 def test_product_is_added(ctx, M, N, K):
     (A, a), (B, b) = _quantized(M, K, 1), _quantized(N, K, 2)
     c = torch.randn(M, N + 4, generator=torch.Generator().manual_seed(3)).to(DEV)

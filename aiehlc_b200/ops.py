@@ -479,8 +479,8 @@ class Context:
             t = None if way == "rows" else MxFp4._of(self._bytes, cols, rows, self.device)
         else:
             q, t = out if way == "both" else (out, None) if way == "rows" else (None, out)
-            for m, r, c in ((q, rows, cols), (t, cols, rows)):
-                if m is not None:
+            for m, r, c, other in ((q, rows, cols, "columns"), (t, cols, rows, "rows")):
+                if way != other:
                     self._mx(m, "out")
                     if m.rows != r or m.cols != c:
                         raise ValueError("quantize_mxfp4: out has other sizes")

@@ -142,7 +142,8 @@ long long aiehlc_mxfp4_scale_bytes(long long rows, long long cols);  /* 512 * ce
  *   along its rows into q, q_scales                  (NULL, NULL: not wanted)
  *   along its columns into t, t_scales, as the transposed matrix [cols][rows] with blocks of 32 rows of x
  *                                                    (NULL, NULL: not wanted)
- * The second is what a product over the rows of x takes: gradients by weights and by activations. */
+ * The second is what a product over the rows of x takes: gradients by weights and by activations.  The outputs overlap
+ * neither x nor one another. */
 int aiehlc_quantize_mxfp4_dev(aiehlc_ctx* ctx, const void* x, int type, long long rows, long long cols, long long ld,
                               uint8_t* q, uint8_t* q_scales, uint8_t* t, uint8_t* t_scales, void* stream);
 /* The values of a quantised matrix, y [rows][cols] of `type`, row pitch `ld` elements.  Exact in f32 and bf16; f16

@@ -470,6 +470,8 @@ def test_refusals(ctx):
     with pytest.raises(ValueError, match="other sizes"):
         ctx.quantize_mxfp4(x, out=MxFp4.empty(40, 65, DEV))
     with pytest.raises(TypeError, match="MxFp4"):
+        ctx.quantize_mxfp4(x, "both", out=(None, MxFp4.empty(64, 40, DEV)))
+    with pytest.raises(TypeError, match="MxFp4"):
         ctx.gemm_mxfp4(x, q)
     with pytest.raises(ValueError, match="K differs"):
         ctx.gemm_mxfp4(q, other)

@@ -300,6 +300,30 @@ class Context:
         fn, check = self._lib.aiehlc_conv2d_i8_srs_dev, _capi.check
         return lambda: check(fn(*args))
 
+    def bound_quantize_mxfp4(self, x, out, way: str = "rows"):
+        """The call quantize_mxfp4(x, way, out), checked and converted once; it keeps its matrices alive."""
+        if self._torch is None:
+            self._mx_setup()
+        if out is None:
+            raise ValueError("bound_quantize_mxfp4: needs an output")
+        args = (self._h, *self._quantize_args(x, way, out)[0], self._raw_stream(self.device))
+        fn, check, keep = self._lib.aiehlc_quantize_mxfp4_dev, _capi.check, (x, out)
+        return lambda _keep=keep: check(fn(*args))
+
+    def bound_gemm_mxfp4(self, A, B, out, accumulate: bool = False):
+        """The call gemm_mxfp4(A, B, out=out, accumulate=accumulate), checked and converted once; it keeps its matrices alive."""
+        if self._torch is None:
+            self._mx_setup()
+        if out is None:
+            raise ValueError("bound_gemm_mxfp4: needs an output")
+        ab = (*self._mx(A, "A"), *self._mx(B, "B"))
+        if A.cols != B.cols:
+            raise ValueError("gemm_mxfp4: A is [M][K], B is [N][K]; K differs")
+        out, addr, kind, ldc = self._result(out, None, A.rows, B.rows, "gemm_mxfp4")
+        args = (self._h, *ab, addr, kind, A.rows, B.rows, A.cols, ldc, 1 if accumulate else 0, self._raw_stream(self.device))
+        fn, check, keep = self._lib.aiehlc_gemm_mxfp4_dev, _capi.check, (A, B, out)
+        return lambda _keep=keep: check(fn(*args))
+
     # --------------------------------------------------------- device tensors
     def mm_i32(self, packed, M: int, N: int, K: int, out=None):
         """The reference's `perf` / `mm` kernel: packed = A (M*K int32) then B (N*K int32)."""
@@ -465,12 +489,7 @@ class Context:
             raise ValueError(f"{name}: the elements of a row must be contiguous and rows must not overlap")
         return t.data_ptr(), kind, rows, cols, ld
 
-    def quantize_mxfp4(self, x, way: str = "rows", out=None):
-        """x [rows][cols] (float32, bfloat16 or float16; rows dense, any row pitch) as MxFp4: along its "rows"; along its
-        "columns" (the transposed matrix [cols][rows], its blocks 32 rows of x, which is what products over the rows of x
-        take); or "both", a pair, from one reading."""
-        if self._torch is None:
-            self._mx_setup()
+    def _quantize_args(self, x, way, out):
         if way not in ("rows", "columns", "both"):
             raise ValueError('quantize_mxfp4: way is "rows", "columns" or "both"')
         addr, kind, rows, cols, ld = self._rows_of(x, "x")
@@ -486,7 +505,16 @@ class Context:
                         raise ValueError("quantize_mxfp4: out has other sizes")
         qc, qs = q._at if q is not None else (None, None)
         tc, ts = t._at if t is not None else (None, None)
-        rc = self._lib.aiehlc_quantize_mxfp4_dev(self._h, addr, kind, rows, cols, ld, qc, qs, tc, ts, self._raw_stream(self.device))
+        return (addr, kind, rows, cols, ld, qc, qs, tc, ts), q, t
+
+    def quantize_mxfp4(self, x, way: str = "rows", out=None):
+        """x [rows][cols] (float32, bfloat16 or float16; rows dense, any row pitch) as MxFp4: along its "rows"; along its
+        "columns" (the transposed matrix [cols][rows], its blocks 32 rows of x, which is what products over the rows of x
+        take); or "both", a pair, from one reading."""
+        if self._torch is None:
+            self._mx_setup()
+        args, q, t = self._quantize_args(x, way, out)
+        rc = self._lib.aiehlc_quantize_mxfp4_dev(self._h, *args, self._raw_stream(self.device))
         if rc:
             _capi.check(rc)
         return (q, t) if way == "both" else q if way == "rows" else t

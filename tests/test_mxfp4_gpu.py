@@ -391,6 +391,36 @@ def test_among_other_kernels_without_a_pause(ctx):
         assert all(torch.equal(x, y) for x, y in zip((c, d, f, g), (outs[0][i] for i in (0, 1, 3, 4))))
 
 
+def test_bound_calls(ctx):
+    """The calls with their arguments converted once, as the other products have them."""
+    x = _matrix(70, 300, 1).float().to(DEV)
+    (W, w) = _whole(200, 300, 2)
+    r, c = _poisoned(70, 300), _poisoned(300, 70)
+    out = torch.empty(70, 200, device=DEV)
+    both, rows, columns = (ctx.bound_quantize_mxfp4(x, o, way) for o, way in (((r, c), "both"), (r, "rows"), (c, "columns")))
+    product, adding = ctx.bound_gemm_mxfp4(r, W, out), ctx.bound_gemm_mxfp4(r, W, out, accumulate=True)
+    before = ctx.launch_count
+    both()
+    _same(r, x.double().cpu().numpy())
+    _same(c, np.ascontiguousarray(x.double().cpu().numpy().T))
+    x.mul_(-2)
+    rows(), columns(), product()
+    _same(c, np.ascontiguousarray(x.double().cpu().numpy().T))
+    want = ctx.gemm_mxfp4(ctx.quantize_mxfp4(x), W, torch.float32)
+    assert torch.equal(out, want)
+    adding()
+    assert torch.equal(out, 2 * want) and ctx.launch_count == before + 7 and ctx.sync() == 0
+    for bind in (lambda: ctx.bound_quantize_mxfp4(x, None), lambda: ctx.bound_gemm_mxfp4(r, W, None)):
+        with pytest.raises(ValueError, match="needs an output"):
+            bind()
+    with pytest.raises(ValueError, match="K differs"):
+        ctx.bound_gemm_mxfp4(c, W, out)
+    with pytest.raises(ValueError, match="shape or type"):
+        ctx.bound_gemm_mxfp4(r, W, out[:69])
+    with pytest.raises(ValueError, match="other sizes"):
+        ctx.bound_quantize_mxfp4(x, c)
+
+
 def test_two_streams_at_once(ctx):
     sets = [_whole(m, 1030, m) + _whole(700, 1030, m + 1) for m in (5, 300, 40, 1000)]
     streams = [torch.cuda.Stream() for _ in sets]

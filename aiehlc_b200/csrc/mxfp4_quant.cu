@@ -335,6 +335,7 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
   }
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
+    if (p * kRowsPerPass >= rows_here) break;
     const int r = p * kRowsPerPass + line;
     const float scale = mx_scale_value(s[p]);
     __half2 h[4];

@@ -34,6 +34,16 @@ template <> __device__ __forceinline__ float2 split2<__nv_bfloat16>(uint32_t w) 
 template <> __device__ __forceinline__ float2 split2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+// Two results to a pair, each rounded to nearest even, in one conversion.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 // Largest magnitude as float bits; a NaN or infinity keeps the exponent 255.
 template <typename T, int kCount>
 __device__ __forceinline__ uint32_t max_bits(const Run<T, kCount>& v) {
@@ -322,19 +332,20 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
   const int cols_here = static_cast<int>(min(static_cast<long long>(kTile), cols - c0));
   const bool col_there = sub * 8 < cols_here;
   const long long pitch = mx_pitch(cols);
-  const uint8_t* src = q + r0 * pitch + c0 / 2 + sub * 4;
+  const uint8_t* src = q + (r0 + line) * pitch + c0 / 2 + sub * 4;
   const uint8_t* scales = qs + (row_tile * mx_words(cols) + col_tile) * kMxScaleTile + sub / 4;
   uint32_t codes[kPasses];
   int s[kPasses];
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
+  for (int p = 0; p < kPasses; ++p, src += kRowsPerPass * pitch) {
     const int r = p * kRowsPerPass + line;
     const bool there = r < rows_here && col_there;
-    codes[p] = there ? *reinterpret_cast<const uint32_t*>(src + r * pitch) : 0u;
+    codes[p] = there ? *reinterpret_cast<const uint32_t*>(src) : 0u;
     s[p] = there ? scales[mx_scale_word(r)] : 0;
   }
+  T* row = y + (r0 + line) * ld + c0 + sub * 8;
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
+  for (int p = 0; p < kPasses; ++p, row += kRowsPerPass * ld) {
     if (p * kRowsPerPass >= rows_here) break;
     const int r = p * kRowsPerPass + line;
     const float scale = mx_scale_value(s[p]);
@@ -344,11 +355,15 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = __half22float2(h[i]);
-      v[2 * i] = mx_from_float<T>(f.x * scale);
-      v[2 * i + 1] = mx_from_float<T>(f.y * scale);
+      if constexpr (sizeof(T) == 4) {
+        v[2 * i] = f.x * scale;
+        v[2 * i + 1] = f.y * scale;
+      } else {
+        reinterpret_cast<uint32_t*>(v)[i] = pack2<T>(f.x * scale, f.y * scale);
+      }
     }
     if constexpr (!kTurn) {
-      T* dst = y + (r0 + r) * ld + c0 + sub * 8;
+      T* dst = row;
       if (r < rows_here && col_there) {
         if (sub * 8 + 8 <= cols_here) {
 #pragma unroll
